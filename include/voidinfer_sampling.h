@@ -393,6 +393,198 @@ vi_status vi_verify_rows(int mode, const void* target, int target_dtype,
                          int32_t* committed_count, uint32_t* lane_flags,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- logit rules: penalties, biases, grammar masks ---------------------------
+ * New entry (the reference has neither biases nor masks): rows of logits
+ * rewritten before a decision.  Every entry point that takes logits, the
+ * verification's included, can be fed from it.  Token t of row r, whose lane is
+ * l = row_lanes[r] (r itself when row_lanes is NULL):
+ *   n  = occurrences of t in lane l's history or penalty state, plus those in
+ *        the row's extra tokens (a drafted row's: the drafted tokens before it)
+ *   x' = n > 0 ? (x > 0 ? x/rep : x*rep) - freq*n - presence : x
+ *                                                 (as vi_row_params, in fp32)
+ *   x' = x' + bias of t in lane l's list, if it has one (of a repeated id the
+ *        last entry counts)
+ *   out = -Inf where the row's mask has bit t clear, else x' rounded once to the
+ *        logit type; logits that no rule touches keep their bits.
+ * A mask is ceil(vocabulary / 32) words, bit t % 32 of word t / 32; a row with
+ * mask_index < 0 (or mask_index NULL) has none.  All pointers are device memory;
+ * NULL lists are empty.  With `params` NULL there are no penalties.  A lane's
+ * history and its penalty state exclude one another (VI_ERR_INVALID for both).
+ * A row that cannot be done (lane outside [0, lanes), mask_index >= masks, a
+ * penalty state with VI_FLAG_ERROR) is written -Inf throughout, so that every
+ * decision over it reports VI_FLAG_EMPTY, and gets VI_FLAG_ERROR in row_flags
+ * (optional, one word per row); history, extra or bias tokens outside
+ * [0, vocabulary) are ignored and set VI_FLAG_BAD_HISTORY.  `out` may be
+ * `logits` itself with the same stride (in place); otherwise the two must not
+ * overlap. */
+typedef struct vi_logit_rules {
+    const vi_row_params* params;        /* [lanes], penalties only, or NULL            */
+    const int32_t* row_lanes;           /* [rows] or NULL                              */
+    const int32_t* histories;           /* histories[history_offsets[l] ..             */
+    const int64_t* history_offsets;     /*   history_offsets[l + 1]), or NULL          */
+    const void* states;                 /* per-lane penalty states, or NULL            */
+    const int32_t* extra;               /* per row: extra[extra_offsets[r] ..          */
+    const int64_t* extra_offsets;       /*   extra_offsets[r + 1]), or NULL            */
+    const int32_t* bias_ids;            /* per lane: bias_offsets[l] ..                */
+    const float* bias_values;           /*   bias_offsets[l + 1], or NULL              */
+    const int64_t* bias_offsets;
+    const uint32_t* mask_words;         /* [masks][mask_stride] or NULL                */
+    const int32_t* mask_index;          /* [rows] or NULL                              */
+    int64_t mask_stride;                /* words, >= ceil(vocabulary / 32)             */
+    int32_t lanes, masks, slots;        /* slots: of the penalty states                */
+    int32_t reserved;
+} vi_logit_rules;
+vi_status vi_process_logits(const void* logits, int dtype, int rows, int vocabulary, int64_t row_stride,
+                            const vi_logit_rules* rules, void* out, int64_t out_stride, uint32_t* row_flags,
+                            void* stream);
+
+/* ---- paged cache of keys and values --------------------------------------------
+ * New entries: what a verification round does to the lanes' caches around the
+ * decision.  A page holds page_size tokens of every kv head; lane l's token i
+ * lies in page tables[l][i / page_size] at place i % page_size.  Page ids are
+ * checked against [0, pages) on the device before any access. */
+typedef struct vi_kv_cache {            /* one layer's pages                           */
+    void* keys;                         /* element (page, head, place, d) at           */
+    void* values;                       /*   page * page_stride + head * head_stride   */
+                                        /*   + place * token_stride + d                */
+    int64_t page_stride, head_stride, token_stride;  /* elements, multiples of 8       */
+    int32_t dtype;                      /* VI_BF16 or VI_F16                           */
+    int32_t pages, page_size;           /* page_size: a power of two, 16 .. 256        */
+    int32_t kv_heads, head_dim;         /* head_dim contiguous elements                */
+    int32_t reserved;
+} vi_kv_cache;
+typedef struct vi_lane_rows {           /* the rows of a call, lane after lane         */
+    const int32_t* row_offsets;         /* device int32[lanes + 1], from 0, ascending  */
+    const int32_t* context;             /* device int32[lanes]: tokens before the rows */
+    const int32_t* tables;              /* device int32[lanes][table_stride]           */
+    int64_t table_stride;               /* entries, >= table_width                     */
+    int32_t table_width, lanes, rows;
+    int32_t reserved;
+} vi_lane_rows;
+
+/* Norm, rotation and append in one pass over the rows' queries, keys and values
+ * ([rows][heads][head_dim] by row and head strides, in elements, 16-byte aligned,
+ * multiples of 8).  Per head vector x of a query or a key:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        (weight NULL: y = x)
+ * and the first rotary_dim elements turn by the row's angles (half = rotary_dim/2,
+ * pair i = (y[i], y[i + half]), or (y[2i], y[2i+1]) when interleaved):
+ *   (a cos_i - b sin_i, a sin_i + b cos_i)
+ * in fp32, rounded once to the element type.  cosines / sines: fp32
+ * [angle_rows][half]; row r takes angle row positions[r], or its cache index when
+ * positions is NULL.  Row r of lane l (i-th of the lane's) has cache index
+ * context[l] + i: queries go to `out`, keys (normed, rotated) and values to the
+ * lane's page.  Rows at or past row_offsets[lanes] are left alone.  A row that
+ * cannot be placed (no valid page, angle row out of range) writes no page, gets
+ * NaN queries and VI_FLAG_ERROR in row_flags (optional, one word per row; 0
+ * otherwise).  rotary_dim: 0 or a multiple of 16, at most head_dim; head_dim: a
+ * multiple of 16, 16 .. 512.  `out` may be the queries themselves with the same
+ * strides. */
+typedef struct vi_head_rows {
+    const void* data;
+    int64_t row_stride, head_stride;
+} vi_head_rows;
+typedef struct vi_rotation {
+    const float* cosines;
+    const float* sines;
+    const int32_t* positions;           /* device int32[rows] or NULL                  */
+    int32_t angle_rows, rotary_dim, interleaved;
+    int32_t reserved;
+} vi_rotation;
+vi_status vi_norm_rotate_append(const vi_kv_cache* cache, const vi_lane_rows* lanes, int heads,
+                                const vi_head_rows* queries, const vi_head_rows* keys, const vi_head_rows* values,
+                                const void* query_weight, const void* key_weight, float eps,
+                                const vi_rotation* rotation, void* out, int64_t out_row_stride,
+                                int64_t out_head_stride, uint32_t* row_flags, void* stream);
+
+/* Attention of the lanes' rows over their pages, the rows' own keys and values
+ * (already appended) included: out = softmax(scale * q k^T) v per query head, kv
+ * head = head / (heads / kv_heads).  Row i of lane l sees the lane's first
+ * context[l] tokens and, of the lane's rows, those up to itself, or with `tree`
+ * (device uint64[rows]) those whose bit is set in tree[row] (bit j: the lane's
+ * row j; lanes of at most 64 rows; a row that does not see itself is allowed).
+ * Groups: lanes group_offsets[g] .. group_offsets[g + 1] (device int32[groups + 1],
+ * from 0 to lanes) share their first prefix_lens[g] tokens (device int32[groups],
+ * at most every such lane's context): these are read through the first lane's
+ * table once for all of the group's rows.  groups 0: nothing is shared.  lse
+ * (optional, fp32 [rows][heads]): log of the sum of exp(scale * q k^T).  A row
+ * that sees no token gets zeros and an lse of -Inf.  A row that sees a token whose
+ * page is not in [0, pages) gets NaN.
+ * The bounds max_rows (rows of a lane), max_group_rows (rows of a group), max_own
+ * (tokens of a lane past its group's prefix, its rows included) and max_prefix
+ * choose the split of the work and size the workspace; lengths past max_own or
+ * max_prefix are still read, rows past max_rows or max_group_rows get NaN.
+ * head_dim: 64, 128 or 256; bf16 or fp16. */
+size_t vi_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int lanes, int groups,
+                                           int max_rows, int max_group_rows, int64_t max_own, int64_t max_prefix);
+vi_status vi_prefix_attention(const vi_kv_cache* cache, const vi_lane_rows* lanes, int heads,
+                              const vi_head_rows* queries, float scale, int groups, const int32_t* group_offsets,
+                              const int32_t* prefix_lens, int max_rows, int max_group_rows, int64_t max_own,
+                              int64_t max_prefix, const uint64_t* tree, void* out, int64_t out_row_stride,
+                              int64_t out_head_stride, float* lse, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Who holds which page: device arrays of the caller.  refs[p] counts the lanes
+ * that hold page p (0: free); tables[l][j] is lane l's j-th page or -1; lengths[l]
+ * its tokens, in ceil(lengths[l] / page_size) pages.  Calls run in stream order.
+ * Arrays that a call does not use may be NULL (compact: lengths; keep_rows: refs
+ * and lengths; status everywhere).
+ * Lane lists (device int32[count], at most 4,096 entries; lanes at most 65,536)
+ * name each lane at most once.  `status` (device int32[3], zeroed by the caller):
+ * [0] VI_FLAG_ERROR once a call was refused on the device, until the caller clears
+ * it; [1], [2] written by extend (pages taken, pages copied) and by compact (live
+ * pages, pages moved). */
+typedef struct vi_page_map {
+    int32_t* refs;
+    int32_t* tables;
+    int32_t* lengths;
+    int32_t* status;
+    int64_t table_stride;               /* entries, >= table_width                     */
+    int32_t pages, page_size;           /* page_size: a power of two, 16 .. 256        */
+    int32_t lanes, table_width;
+} vi_page_map;
+/* The page contents of all layers: page p of plane i (a layer's keys, or its
+ * values) at base + i * plane_stride + p * page_bytes, in bytes, multiples of 16. */
+typedef struct vi_page_pool {
+    void* base;
+    int64_t plane_stride, page_bytes;
+    int32_t planes, reserved;
+} vi_page_pool;
+/* children[i] gives back what it held and takes parents[i]'s pages and length.  A
+ * child that is listed twice or is itself a parent in the call is left as it was. */
+vi_status vi_pages_fork(const vi_page_map* map, const int32_t* parents, const int32_t* children, int count,
+                        void* stream);
+/* lane_ids[i] grows to new_lengths[i] >= lengths: the pages that it lacks are the
+ * lowest free ones, in list order.  Where a growing lane's last page is partly
+ * filled and other lanes hold it too, the lane gets a copy of its own first (its
+ * first new page; of the listed lanes that share one, the last keeps the page
+ * when no other lane holds it).  All or nothing: too few free pages, a bad lane, a
+ * shrinking length or one past the table changes nothing. */
+size_t vi_pages_extend_workspace_bytes(int count);
+vi_status vi_pages_extend(const vi_page_map* map, const vi_page_pool* pool, const int32_t* lane_ids,
+                          const int32_t* new_lengths, int count, void* workspace, size_t workspace_bytes,
+                          void* stream);
+/* lane_ids[i] shrinks to new_lengths[i] (0: the lane is free); a length that is not
+ * smaller leaves the lane as it is. */
+vi_status vi_pages_truncate(const vi_page_map* map, const int32_t* lane_ids, const int32_t* new_lengths, int count,
+                            void* stream);
+/* Page sources[i] to page targets[i] in every plane; no target is listed twice or
+ * is a source.  Ids outside [0, pages) are skipped. */
+vi_status vi_pages_copy(const vi_page_pool* pool, int pages, const int32_t* sources, const int32_t* targets,
+                        int count, void* stream);
+/* The pool's n live pages move to the ids below n: the k-th free id below n takes
+ * the k-th live page above, in ascending order; tables and refs follow. */
+size_t vi_pages_compact_workspace_bytes(int pages);
+vi_status vi_pages_compact(const vi_page_map* map, const vi_page_pool* pool, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* Of the rows a lane appended at context[i], the accepted path stays: row
+ * paths[i][j] moves to cache index context[i] + j, for j < kept[i] (paths: device
+ * int32[count][path_stride], ascending, paths[i][j] >= j).  Entries that are not
+ * so, or whose pages are not valid, are skipped.  Pages are [kv_heads][page_size]
+ * rows of page_bytes / (kv_heads * page_size) bytes, a multiple of 16. */
+vi_status vi_keep_rows(const vi_page_map* map, const vi_page_pool* pool, int kv_heads, const int32_t* lane_ids,
+                       const int32_t* context, const int32_t* paths, int path_stride, const int32_t* kept,
+                       int count, void* stream);
+
 /* ---- measurement helpers ------------------------------------------------------
  * Stream-read probe (the gfx950 analogue of tools/hbm_bandwidth_probe.cu:1-45):
  * reads `bytes` from `src` with 16-byte loads and writes one word per

@@ -1,0 +1,212 @@
+"""Refusals of the logit rules and of the paged cache's entry points, on the CPU:
+the arguments are checked on the host before any launch, so no GPU is needed and
+the (never read) device pointers are made up."""
+import pytest
+import torch
+
+INVALID, UNSUPPORTED, OK = 1, 2, 0
+P = 4096   # a 16-byte aligned address that no accepted call is given here
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from voidinfer_amd import _abi
+    return _abi.load()
+
+
+def rules(**kw):
+    from voidinfer_amd import _abi
+    f = dict(params=P, row_lanes=0, histories=0, history_offsets=0, states=0, extra=0, extra_offsets=0, bias_ids=0,
+             bias_values=0, bias_offsets=0, mask_words=0, mask_index=0, mask_stride=0, lanes=4, masks=0, slots=0)
+    assert not set(kw) - set(f)
+    f.update(kw)
+    return _abi.LOGIT_RULES.pack(*f.values(), 0)
+
+
+@pytest.mark.parametrize("args,kw", [
+    (dict(rows=-1), {}), (dict(vocab=0), {}), (dict(stride=99), {}), (dict(out_stride=99), {}), (dict(dtype=3), {}),
+    (dict(logits=0), {}), (dict(out=0), {}), (dict(out_stride=128, out=P), {}),
+    ({}, dict(lanes=0)), (dict(rows=5), {}),
+    ({}, dict(histories=P)), ({}, dict(histories=P, history_offsets=P, states=P, slots=64)), ({}, dict(extra=P)),
+    ({}, dict(bias_ids=P, bias_values=P)), ({}, dict(bias_ids=P, bias_offsets=P)), ({}, dict(states=P, slots=63)),
+    ({}, dict(mask_index=P)), ({}, dict(mask_index=P, mask_words=P, masks=2, mask_stride=3)),
+    ({}, dict(mask_index=P, mask_words=P, masks=0, mask_stride=4)),
+])
+def test_process_logits_refuses(lib, args, kw):
+    a = dict(logits=P, dtype=0, rows=4, vocab=100, stride=100, out=2 * P, out_stride=100)
+    a.update(args)
+    assert lib.vi_process_logits(a["logits"], a["dtype"], a["rows"], a["vocab"], a["stride"], rules(**kw), a["out"],
+                                 a["out_stride"], 0, 0) == INVALID
+
+
+def test_no_rows_is_no_work(lib):
+    assert lib.vi_process_logits(0, 0, 0, 100, 100, rules(), 0, 100, 0, 0) == OK
+    assert lib.vi_norm_rotate_append(cache(), lane_rows(rows=0), 8, heads(), heads(), heads(), 0, 0, 1e-6, rotation(),
+                                     P, 0, 0, 0, 0) == OK
+    for f in (lib.vi_pages_fork, lib.vi_pages_truncate):
+        assert f(page_map(), 0, 0, 0, 0) == OK
+    assert lib.vi_pages_copy(pool(), 10, 0, 0, 0, 0) == OK
+
+
+def cache(**kw):
+    from voidinfer_amd import _abi
+    f = dict(keys=P, values=P, page_stride=4 * 16 * 128, head_stride=16 * 128, token_stride=128, dtype=0, pages=10,
+             page_size=16, kv_heads=4, head_dim=128)
+    assert not set(kw) - set(f)
+    f.update(kw)
+    return _abi.KV_CACHE.pack(*f.values(), 0)
+
+
+def lane_rows(**kw):
+    from voidinfer_amd import _abi
+    f = dict(row_offsets=P, context=P, tables=P, table_stride=8, table_width=8, lanes=2, rows=4)
+    assert not set(kw) - set(f)
+    f.update(kw)
+    return _abi.LANE_ROWS.pack(*f.values(), 0)
+
+
+def heads(**kw):
+    from voidinfer_amd import _abi
+    f = dict(data=P, row_stride=1024, head_stride=128)
+    f.update(kw)
+    return _abi.HEAD_ROWS.pack(*f.values())
+
+
+def rotation(**kw):
+    from voidinfer_amd import _abi
+    f = dict(cosines=P, sines=P, positions=0, angle_rows=10, rotary_dim=128, interleaved=0)
+    f.update(kw)
+    return _abi.ROTATION.pack(*f.values(), 0)
+
+
+CACHE_FAULTS = [
+    (INVALID, dict(keys=0)), (INVALID, dict(values=0)), (INVALID, dict(keys=P + 8)), (INVALID, dict(pages=0)),
+    (INVALID, dict(page_size=24)), (INVALID, dict(page_size=8)), (INVALID, dict(page_size=512)),
+    (INVALID, dict(kv_heads=3)), (INVALID, dict(token_stride=132)), (INVALID, dict(head_stride=-8)),
+    (INVALID, dict(dtype=5)), (UNSUPPORTED, dict(dtype=2)),
+]
+LANE_FAULTS = [dict(row_offsets=0), dict(context=0), dict(tables=0), dict(table_stride=7), dict(table_width=0),
+               dict(lanes=0), dict(rows=-1)]
+
+
+@pytest.mark.parametrize("want,kw", CACHE_FAULTS + [(UNSUPPORTED, dict(head_dim=24)), (UNSUPPORTED, dict(head_dim=528))])
+def test_append_refuses_caches(lib, want, kw):
+    rot = rotation(rotary_dim=16)
+    assert lib.vi_norm_rotate_append(cache(**kw), lane_rows(), 8, heads(), heads(), heads(), 0, 0, 1e-6, rot, P, 1024,
+                                     128, 0, 0) == want
+
+
+@pytest.mark.parametrize("want,kw", CACHE_FAULTS + [(UNSUPPORTED, dict(head_dim=96))])
+def test_attention_refuses_caches(lib, want, kw):
+    assert lib.vi_prefix_attention(cache(**kw), lane_rows(), 8, heads(), 0.1, 0, 0, 0, 4, 0, 10, 0, 0, P, 1024, 128, 0,
+                                   P, 1 << 30, 0) == want
+
+
+@pytest.mark.parametrize("kw", LANE_FAULTS)
+def test_lane_rows_refused(lib, kw):
+    l = lane_rows(**kw)
+    assert lib.vi_norm_rotate_append(cache(), l, 8, heads(), heads(), heads(), 0, 0, 1e-6, rotation(), P, 1024, 128, 0,
+                                     0) == INVALID
+    assert lib.vi_prefix_attention(cache(), l, 8, heads(), 0.1, 0, 0, 0, 4, 0, 10, 0, 0, P, 1024, 128, 0, P, 1 << 30,
+                                   0) == INVALID
+
+
+@pytest.mark.parametrize("want,kw", [
+    (INVALID, dict(q=heads(data=0))), (INVALID, dict(q=heads(data=P + 2))), (INVALID, dict(k=heads(row_stride=1028))),
+    (INVALID, dict(v=heads(head_stride=-8))), (INVALID, dict(out=0)), (INVALID, dict(out=P + 8)),
+    (INVALID, dict(out_row=1020)), (INVALID, dict(eps=float("nan"))), (INVALID, dict(eps=-1.0)),
+    (INVALID, dict(weight=P + 2)), (INVALID, dict(rot=rotation(rotary_dim=144))), (INVALID, dict(heads=6)),
+    (INVALID, dict(rot=rotation(cosines=0))), (INVALID, dict(rot=rotation(angle_rows=0))),
+    (UNSUPPORTED, dict(rot=rotation(rotary_dim=24))),
+])
+def test_append_refuses(lib, want, kw):
+    a = dict(heads=8, q=heads(), k=heads(), v=heads(), weight=0, eps=1e-6, rot=rotation(), out=P, out_row=1024)
+    a.update(kw)
+    assert lib.vi_norm_rotate_append(cache(), lane_rows(), a["heads"], a["q"], a["k"], a["v"], a["weight"], 0,
+                                     a["eps"], a["rot"], a["out"], a["out_row"], 128, 0, 0) == want
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=heads(data=P + 2)), dict(out=0), dict(groups=-1), dict(groups=3, go=P, pl=P, group_rows=4),
+    dict(groups=1, pl=P, group_rows=4), dict(groups=1, go=P, group_rows=4), dict(groups=1, go=P, pl=P),
+    dict(max_rows=0), dict(max_own=-1), dict(max_prefix=-1), dict(scale=float("nan")), dict(heads=7),
+])
+def test_attention_refuses(lib, kw):
+    a = dict(heads=8, q=heads(), scale=0.1, groups=0, go=0, pl=0, max_rows=4, group_rows=0, max_own=10, max_prefix=0,
+             out=P)
+    a.update(kw)
+    assert lib.vi_prefix_attention(cache(), lane_rows(), a["heads"], a["q"], a["scale"], a["groups"], a["go"], a["pl"],
+                                   a["max_rows"], a["group_rows"], a["max_own"], a["max_prefix"], 0, a["out"], 1024,
+                                   128, 0, P, 1 << 30, 0) == INVALID
+
+
+def page_map(**kw):
+    from voidinfer_amd import _abi
+    f = dict(refs=P, tables=P, lengths=P, status=P, table_stride=8, pages=10, page_size=16, lanes=4, table_width=8)
+    assert not set(kw) - set(f)
+    f.update(kw)
+    return _abi.PAGE_MAP.pack(*f.values())
+
+
+def pool(**kw):
+    from voidinfer_amd import _abi
+    f = dict(base=P, plane_stride=10 * 4096, page_bytes=4096, planes=2)
+    f.update(kw)
+    return _abi.PAGE_POOL.pack(*f.values(), 0)
+
+
+MAP_FAULTS = [(INVALID, dict(refs=0)), (INVALID, dict(tables=0)), (INVALID, dict(lengths=0)), (INVALID, dict(pages=0)),
+              (INVALID, dict(lanes=0)), (INVALID, dict(table_width=0)), (INVALID, dict(table_stride=7)),
+              (INVALID, dict(page_size=20)), (UNSUPPORTED, dict(lanes=65537))]
+
+
+@pytest.mark.parametrize("want,kw", MAP_FAULTS)
+def test_page_maps_refused(lib, want, kw):
+    m = page_map(**kw)
+    assert lib.vi_pages_fork(m, P, P, 2, 0) == want
+    assert lib.vi_pages_truncate(m, P, P, 2, 0) == want
+    assert lib.vi_pages_extend(m, pool(), P, P, 2, P, 1 << 20, 0) == want
+    if "lengths" not in kw:
+        assert lib.vi_pages_compact(m, pool(), P, 1 << 20, 0) == want
+
+
+@pytest.mark.parametrize("kw", [dict(base=0), dict(base=P + 8), dict(planes=0), dict(page_bytes=24), dict(page_bytes=0),
+                                dict(plane_stride=-16), dict(plane_stride=8)])
+def test_pools_refused(lib, kw):
+    assert lib.vi_pages_extend(page_map(), pool(**kw), P, P, 2, P, 1 << 20, 0) == INVALID
+    assert lib.vi_pages_compact(page_map(), pool(**kw), P, 1 << 20, 0) == INVALID
+    assert lib.vi_pages_copy(pool(**kw), 10, P, P, 2, 0) == INVALID
+    assert lib.vi_keep_rows(page_map(), pool(**kw), 4, P, P, P, 4, P, 2, 0) == INVALID
+
+
+def test_page_calls_refuse(lib):
+    assert lib.vi_pages_fork(page_map(), 0, P, 2, 0) == INVALID
+    assert lib.vi_pages_fork(page_map(), P, P, -1, 0) == INVALID
+    assert lib.vi_pages_truncate(page_map(), P, P, 4097, 0) == UNSUPPORTED
+    assert lib.vi_pages_copy(pool(), 0, P, P, 2, 0) == INVALID
+    assert lib.vi_keep_rows(page_map(), pool(), 0, P, P, P, 4, P, 2, 0) == INVALID
+    assert lib.vi_keep_rows(page_map(), pool(), 5, P, P, P, 4, P, 2, 0) == INVALID    # 4,096 / (5 heads x 16 places)
+    assert lib.vi_keep_rows(page_map(), pool(), 4, P, P, P, 0, P, 2, 0) == INVALID
+    # a workspace that is missing or too small
+    assert lib.vi_pages_extend(page_map(), pool(), P, P, 2, 0, 0, 0) == 3
+    assert lib.vi_pages_extend(page_map(), pool(), P, P, 100, P, 256, 0) == 3
+    assert lib.vi_pages_compact(page_map(), pool(), P, 64, 0) == 3
+    assert lib.vi_pages_extend_workspace_bytes(0) == 0 and lib.vi_pages_extend_workspace_bytes(64) > 512
+    assert lib.vi_pages_compact_workspace_bytes(0) == 0 and lib.vi_pages_compact_workspace_bytes(64) > 768
+    assert lib.vi_prefix_attention_workspace_bytes(0, 8, 8, 128, 1, 0, 1, 0, 1, 0) == 0
+    assert lib.vi_prefix_attention_workspace_bytes(4, 8, 8, 128, 1, 0, 1, 0, 100, 0) > 0
+
+
+def test_host_tensors_and_shapes_are_refused():
+    import voidinfer_amd as vi
+    x = torch.zeros(2, 64)
+    with pytest.raises(ValueError):
+        vi.process_logits(x)                                       # not on a device
+    q, pages = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    t, i = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        vi.prefix_attention(q, pages, pages, t, i, i[:1], max_rows=2, max_own=4)
+    with pytest.raises(ValueError):
+        vi.pages_fork(i, t, i[:1], i, i, 16)
+    with pytest.raises(ValueError):
+        vi.pages_copy(pages, i, i)

@@ -1,0 +1,318 @@
+"""vi_prefix_attention against its definition in 64 bits.
+
+Tolerance (u: half a unit in the last place of the element type).  The weights may
+be rounded to the element type before they meet the values (u of sum p |v|, and
+for fp16 2^-25 an entry below its normal range), the result is rounded once (u of
+|out|); the scores are fp32 sums of d products, off by at most (d + 4) 2^-24 of
+scale * sum |q k| =: S, which moves a weight by that factor, and exp, the sums over
+n keys and the joining of parts add a few 2^-24: in all 2^-22 (4 + (d + 4) S + sqrt n)
+of sum p |v|.  The lse is off by (d + 4) 2^-24 S + 2^-22 (1 + |lse|)."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+class Case:
+    """A batch of lanes over random pages; groups: list of (lanes, shared tokens)."""
+
+    def __init__(self, rng, dev, dtype, counts, contexts, heads, kv_heads, dim, page, groups=(), tree=None, spread=1.0,
+                 layout="heads", spare=2):
+        self.dev, self.dtype, self.counts, self.contexts = dev, dtype, list(counts), list(contexts)
+        lanes, self.ps = len(counts), page
+        held = [-(-(c + n) // page) for c, n in zip(contexts, counts)]
+        pages = sum(held) + spare
+        self.tables = np.full((lanes, max(max(held), 1) + 1), -1, dtype=np.int32)
+        order, at = rng.permutation(pages), 0
+        for i, n in enumerate(held):
+            self.tables[i, :n] = order[at:at + n]
+            at += n
+        rand = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+        rows = sum(counts)
+        self.q = (rand(rows, heads, dim) * spread).to(dtype).to(dev)
+        if layout == "heads":
+            self.pool = rand(2, pages, kv_heads, page, dim).to(dtype).to(dev)
+        else:
+            self.pool = rand(2, pages, page, kv_heads, dim).to(dtype).to(dev).transpose(2, 3)
+        self.groups, first = groups, 0
+        for n, shared in groups:   # the lanes' first tokens are alike: whole pages shared, the last one copied
+            for l in range(first + 1, first + n):
+                whole = shared // page
+                self.tables[l, :whole] = self.tables[first, :whole]
+                if shared % page:
+                    a, b = self.tables[first, whole], self.tables[l, whole]
+                    self.pool[:, b, :, :shared % page] = self.pool[:, a, :, :shared % page]
+            first += n
+        self.tree = tree
+        self.off = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+
+    def i32(self, x):
+        return torch.tensor(np.asarray(x, dtype=np.int32), device=self.dev)
+
+    def run(self, **over):
+        import voidinfer_amd as vi
+        rows, heads, dim = self.q.shape
+        self.lse = torch.full((rows, heads), 7.0, device=self.dev)
+        kw = dict(max_rows=max(self.counts), max_own=max(c + n for c, n in zip(self.contexts, self.counts)), lse=self.lse)
+        if self.groups:
+            ends = np.concatenate([[0], np.cumsum([n for n, _ in self.groups])])
+            rows_of = [sum(self.counts[a:b]) for a, b in zip(ends, ends[1:])]
+            kw |= dict(group_offsets=self.i32(ends), prefix_lens=self.i32([p for _, p in self.groups]),
+                       max_group_rows=max(max(rows_of), 1), max_prefix=max(p for _, p in self.groups))
+        if self.tree is not None:
+            kw["tree"] = torch.tensor(np.asarray(self.tree, dtype=np.uint64).view(np.int64), device=self.dev)
+        kw |= over
+        return vi.prefix_attention(self.q, self.pool[0], self.pool[1], self.i32(self.tables), self.i32(self.off),
+                                   self.i32(self.contexts), **kw)
+
+    def check(self, out, scale=None, skip=()):
+        rows, heads, dim = self.q.shape
+        hk = self.pool.shape[2]
+        g, scale = heads // hk, 1 / np.sqrt(dim) if scale is None else scale
+        q = self.q.double().cpu().numpy()
+        pool = self.pool.double().cpu().numpy()
+        got, lse = out.double().cpu().numpy(), self.lse.double().cpu().numpy()
+        for l, (n, c) in enumerate(zip(self.counts, self.contexts)):
+            if not n or l in skip:
+                continue
+            at = np.arange(c + n)
+            page, place = self.tables[l, at // self.ps], at % self.ps
+            k, v = (np.repeat(x[page, :, place], g, axis=1) for x in pool)          # [keys, heads, dim]
+            for i in range(n):
+                r = self.off[l] + i
+                if self.tree is None:
+                    seen = at <= c + i
+                else:
+                    seen = (at < c) | np.array([t >= c and bool(int(self.tree[r]) >> int(t - c) & 1) for t in at])
+                if not seen.any():
+                    assert (got[r] == 0).all() and np.isneginf(lse[r]).all(), (l, i)
+                    continue
+                prod = q[r][None] * k[seen] * scale
+                s, mass = prod.sum(-1), np.abs(prod).sum(-1).max()
+                top = s.max(0)
+                p = np.exp(s - top)
+                total = p.sum(0)
+                p /= total
+                want, big = np.einsum("kh,khd->hd", p, v[seen]), np.einsum("kh,khd->hd", p, np.abs(v[seen]))
+                u, keys = UNIT[self.dtype], int(seen.sum())
+                bound = (u * 1.01 + 2.0 ** -22 * (4 + (dim + 4) * mass + np.sqrt(keys))) * big + u * np.abs(want) + \
+                    TINY[self.dtype] * (1 + keys * np.abs(v[seen]).max() / total.min())
+                err = np.abs(got[r] - want)
+                assert (err <= bound).all(), (l, i, float((err / bound).max()))
+                want = top + np.log(total)
+                assert (np.abs(lse[r] - want) <= (dim + 4) * 2.0 ** -24 * mass + 2.0 ** -22 * (1 + np.abs(want))).all(), (l, i)
+
+
+BOTH = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+
+
+@BOTH
+@pytest.mark.parametrize("counts,contexts,heads,kv,dim,page", [
+    ([1], [0], 1, 1, 64, 16),                                    # one token, itself alone
+    ([1], [1], 2, 1, 128, 16),
+    ([1, 1, 1, 1], [0, 15, 16, 31], 8, 2, 64, 16),               # ends at, before and behind a page
+    ([1, 1, 1], [63, 64, 65], 4, 4, 128, 64),                    # ... and a tile
+    ([1] * 5, [127, 128, 129, 255, 700], 14, 2, 128, 16),        # 7 heads share a kv head
+    ([1, 1], [1500, 3], 32, 8, 128, 32),
+    ([1], [5000], 8, 1, 256, 16),
+    ([1, 1], [333, 2001], 16, 1, 64, 256),
+    ([17, 3, 1, 0, 8], [100, 0, 700, 40, 31], 8, 2, 128, 16),    # verified blocks, one lane with nothing
+    ([5, 5], [1000, 64], 24, 3, 256, 64),
+    ([130], [0], 4, 2, 64, 16),                                  # a short prompt
+    ([70, 33], [20, 500], 6, 2, 128, 16),
+])
+def test_lanes_alone(dev, rng, dtype, counts, contexts, heads, kv, dim, page):
+    print("attention", dtype, counts, contexts, heads, kv, dim, page, flush=True)
+    c = Case(rng, dev, dtype, counts, contexts, heads, kv, dim, page)
+    c.check(c.run())
+
+
+@BOTH
+@pytest.mark.parametrize("counts,contexts,heads,kv,dim,page,groups", [
+    ([1, 1], [16, 20], 2, 2, 64, 16, [(2, 16)]),                       # one lane has only the prefix and its row
+    ([1] * 4, [64, 70, 90, 129], 8, 2, 64, 16, [(4, 64)]),
+    ([1] * 9, [300 + 7 * i for i in range(9)], 8, 2, 128, 32, [(9, 288)]),
+    ([1] * 6, [40, 41, 42, 200, 201, 202], 4, 1, 128, 16, [(3, 33), (3, 170)]),   # ends inside a page
+    ([1] * 5, [100, 90, 80, 70, 60], 4, 2, 256, 16, [(1, 50), (2, 0), (2, 60)]),  # a group of one, one that shares nothing
+    ([17, 9, 12, 1], [600, 555, 513, 512], 8, 2, 128, 16, [(4, 512)]),
+    ([6, 0, 3], [64, 64, 80], 8, 1, 128, 64, [(3, 64)]),
+    ([1] * 40, [130 + i for i in range(40)], 16, 2, 64, 16, [(40, 128)]),         # many rows of one prefix
+    ([1, 1, 1], [1030, 1024, 1100], 10, 2, 128, 16, [(2, 1024), (1, 1000)]),
+    ([3, 2], [3000, 2950], 32, 2, 128, 16, [(2, 2900)]),
+])
+def test_groups_share_a_prefix(dev, rng, dtype, counts, contexts, heads, kv, dim, page, groups):
+    """The prefix is read through the group's first lane, the answer is that of each lane alone."""
+    print("attention groups", dtype, counts, groups, heads, kv, dim, page, flush=True)
+    c = Case(rng, dev, dtype, counts, contexts, heads, kv, dim, page, groups)
+    out = c.run()
+    c.check(out)
+    own = max(x + n - p for x, n, p in zip(contexts, counts, np.repeat([p for _, p in groups], [n for n, _ in groups])))
+    c.check(c.run(max_own=int(own)))              # the tight bound, and one that is too small: still read whole
+    c.check(c.run(max_own=1, max_prefix=1))
+
+
+@BOTH
+def test_trees(dev, rng, dtype):
+    """Chains, siblings, rows that see nothing of the lane's rows, not even themselves, and with no context
+    nothing at all; 64 rows, the last bit used."""
+    counts, contexts = [9, 3, 64, 2, 17], [40, 0, 77, 0, 200]
+    tree = []
+    for n in counts:
+        for i in range(n):
+            bits = 1 << i
+            for j in range(i):
+                bits |= int(rng.random() < 0.6) << j
+            tree.append(bits)
+    tree[9] = 0                 # lane 1 (no context), row 0: nothing at all
+    tree[5] = 0                 # lane 0, row 5: the context only
+    tree[9 + 3 + 64] = 2        # lane 3 row 0 sees row 1 only (behind it), which ...
+    tree[9 + 3 + 64 + 1] = 0    # ... itself sees nothing
+    tree[9 + 3 + 3] |= 1 << 63
+    for groups in ((), [(1, 30), (1, 0), (1, 64), (1, 0), (1, 200)]):
+        c = Case(rng, dev, dtype, counts, contexts, 8, 2, 128, 16, groups, tree)
+        c.check(c.run())
+    # a chain's masks are the default
+    chain = [(1 << (i + 1)) - 1 for n in counts for i in range(n)]
+    a = Case(rng, dev, dtype, counts, contexts, 8, 2, 128, 16, (), chain)
+    out = a.run()
+    a.tree = None
+    assert torch.equal(out, a.run())
+
+
+@BOTH
+def test_peaked_and_large_scores(dev, rng, dtype):
+    """Scores in the hundreds (one key takes everything), of both signs and a scale of zero: no overflow."""
+    c = Case(rng, dev, dtype, [1, 4], [700, 90], 8, 2, 128, 16, [(2, 80)], spread=60.0)
+    c.check(c.run())
+    c.check(c.run(scale=-0.25), scale=-0.25)
+    c.check(c.run(scale=0.0), scale=0.0)
+
+
+def test_masked_places_may_hold_anything(dev, rng):
+    """NaN and Inf in pages' places behind a lane's tokens, in free pages and in rows that the tree hides leave no trace."""
+    tree = [1, 2, 5, 8 | 1]
+    c = Case(rng, dev, torch.bfloat16, [4, 1], [19, 33], 8, 2, 128, 16, (), tree + [1])
+    for l, n in ((0, 23), (1, 34)):
+        page = c.tables[l, n // 16]
+        c.pool[:, page, :, n % 16:] = float("nan")
+    used = c.tables[c.tables >= 0]
+    free = [p for p in range(c.pool.shape[1]) if p not in used]
+    c.pool[:, free] = float("inf")
+    keep = c.pool[:, c.tables[0, 1], :, 4].clone()
+    c.pool[0, c.tables[0, 1], :, 4] = float("nan")       # row 1's own key (index 20): seen by row 1 alone
+    c.pool[1, c.tables[0, 1], :, 4] = float("inf")
+    out = c.run()
+    assert bool(torch.isnan(out[1]).all())
+    c.pool[:, c.tables[0, 1], :, 4] = keep
+    out[1] = c.run()[1]
+    c.check(out)
+
+
+def test_bad_pages_and_bounds(dev, rng):
+    """A page id out of range among the tokens that a row sees gives NaN (and only there); rows past the bounds too."""
+    c = Case(rng, dev, torch.float16, [2, 1, 3], [100, 50, 20], 4, 2, 64, 16)
+    good = c.run()
+    for bad in (-1, 10_000, -2 ** 31):
+        keep = c.tables[0, 3]
+        c.tables[0, 3] = bad
+        out = c.run()
+        assert bool(torch.isnan(out[:2]).all()) and torch.equal(out[2:], good[2:])
+        c.tables[0, 3] = keep
+    c.tables[1, 4:] = 10_000     # behind the lane's tokens: never read
+    assert torch.equal(c.run(), good)
+    out = c.run(max_rows=2)
+    assert torch.equal(out[:5], good[:5]) and bool(torch.isnan(out[5]).all())
+    g = Case(rng, dev, torch.float16, [2, 1, 3], [100, 100, 100], 4, 2, 64, 16, [(2, 96), (1, 0)])
+    good = g.run()
+    g.check(good)
+    out = g.run(max_group_rows=2)
+    assert bool(torch.isnan(out).all()) or (torch.equal(out[:2], good[:2]) and bool(torch.isnan(out[2]).all()))
+
+
+@BOTH
+def test_strides_and_padding(dev, rng, dtype):
+    """Pages laid out token by token, queries and outputs inside wider rows, rows past the last lane left alone."""
+    c = Case(rng, dev, dtype, [3, 1, 2], [45, 130, 7], 6, 2, 128, 16, [(1, 20), (2, 0)], layout="tokens")
+    want = c.run()
+    c.check(want)
+    wide = torch.full((8, 7, 160), 3.0, dtype=dtype, device=dev)
+    wide[:6, :6, 8:136] = c.q
+    c.q = wide[:, :6, 8:136]
+    out = torch.full((8, 9, 144), 5.0, dtype=dtype, device=dev)
+    c.run(out=out[:, 2:8, 16:])
+    assert torch.equal(out[:6, 2:8, 16:], want)
+    out[:6, 2:8, 16:] = 5
+    assert bool((out == 5).all()) and bool((c.lse[6:] == 7).all())
+
+
+def test_stream_repeats_and_graph(dev, rng):
+    """The same bits on every call, on a stream of its own and from a graph that is replayed."""
+    c = Case(rng, dev, torch.bfloat16, [1] * 12, [600 + i for i in range(12)], 16, 2, 128, 16, [(12, 576)])
+    want = c.run().clone()
+    out = torch.empty_like(want)
+    kw = dict(max_rows=1, max_own=40, max_group_rows=12, max_prefix=576, group_offsets=c.i32([0, 12]),
+              prefix_lens=c.i32([576]), out=out)
+    import voidinfer_amd as vi
+    args = (c.q, c.pool[0], c.pool[1], c.i32(c.tables), c.i32(c.off), c.i32(c.contexts))
+    vi.prefix_attention(*args, **kw)
+    tight = out.clone()
+    c.check(tight)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            out.zero_()
+            vi.prefix_attention(*args, **kw)
+    s.synchronize()
+    assert torch.equal(out, tight)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        vi.prefix_attention(*args, **kw)
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, tight)
+
+
+def test_a_cache_past_32_bits(dev, rng):
+    """Pages whose elements lie past 2^32 bytes (and 2^31 elements) of the pool's base."""
+    c = Case(rng, dev, torch.bfloat16, [1, 1], [200, 330], 8, 2, 128, 16, [(2, 192)])
+    small = c.pool
+    pages = 600_000
+    big = torch.zeros(2, pages, 2, 16, 128, dtype=torch.bfloat16, device=dev)
+    n = small.shape[1]
+    big[:, pages - n:] = small
+    want = c.run()
+    c.tables = np.where(c.tables >= 0, c.tables + (pages - n), -1).astype(np.int32)
+    c.pool = big
+    assert torch.equal(c.run(), want)
+
+
+def test_refusals(dev):
+    import voidinfer_amd as vi
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device=dev)
+    pool = torch.zeros(2, 3, 2, 16, 64, dtype=torch.float16, device=dev)
+    base = (q, pool[0], pool[1], i32([[0, 1]]), i32([0, 2]), i32([0]))
+    ok = dict(max_rows=2, max_own=2)
+    vi.prefix_attention(*base, **ok)
+    for at, bad in ((0, q.bfloat16()), (0, q[:, :3]), (1, pool[0].float()), (2, pool[1, :2]), (3, i32([0])), (4, i32([0])),
+                    (5, i32([0, 1]))):
+        args = list(base)
+        args[at] = bad
+        with pytest.raises(ValueError):
+            vi.prefix_attention(*args, **ok)
+    for kw in (dict(max_rows=0), dict(group_offsets=i32([0, 1])), dict(group_offsets=i32([0, 1]), prefix_lens=i32([0])),
+               dict(tree=i32([1, 1])), dict(lse=torch.zeros(2, 3, device=dev)), dict(out=q[:1]),
+               dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            vi.prefix_attention(*base, **{**ok, **kw})
+    with pytest.raises(vi.VIError):      # a head size that has no kernel
+        vi.prefix_attention(torch.zeros(2, 4, 96, dtype=torch.float16, device=dev), *(torch.zeros(
+            3, 2, 16, 96, dtype=torch.float16, device=dev) for _ in range(2)), *base[3:], **ok)

@@ -1,0 +1,261 @@
+"""vi_process_logits against its definition in 64 bits.
+
+Tolerance: the kernel rounds each fp32 operation (division or product, count
+product, two differences, the bias' sum: at most 5 of them, each at most 2^-24 of
+the largest magnitude that occurs) and the result once to the logit type, at most
+half a unit in the last place.  Logits that no rule touches keep their bits, and
+masked ones are -Inf."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import DT_TORCH
+
+pytestmark = pytest.mark.gpu
+
+FLAG_BAD_HISTORY, FLAG_ERROR = 16, -(1 << 31)
+UNIT = {0: 2.0 ** -8, 1: 2.0 ** -11, 2: 2.0 ** -24}      # half a unit in the last place, relative
+TINY = {0: 0.0, 1: 2.0 ** -25, 2: 0.0}                    # half the smallest step of fp16 near zero
+
+
+def reference(x, params, lane_of, count, bias, allowed):
+    """(values, magnitudes) in float64 from x float64 [rows, vocab]; count / bias [rows, vocab] (bias NaN: none)."""
+    out, big = x.copy(), np.abs(x)
+    for r, l in enumerate(lane_of):
+        rep, pres, freq = (float(params[l][f]) for f in ("repetition_penalty", "presence_penalty", "frequency_penalty"))
+        t = count[r] > 0
+        y = np.where(x[r] > 0, x[r] / rep, x[r] * rep)
+        big[r][t] = np.abs(y)[t] + abs(freq) * count[r][t] + abs(pres)
+        out[r][t] = (y - freq * count[r] - pres)[t]
+        b = ~np.isnan(bias[r])
+        out[r][b] += bias[r][b]
+        big[r][b] += np.abs(bias[r][b])
+    out[~allowed] = -np.inf
+    return out, big
+
+
+def pack(allowed):
+    rows, vocab = allowed.shape
+    words = -(-vocab // 32)
+    bits = np.zeros((rows, words * 32), dtype=np.uint8)
+    bits[:, :vocab] = allowed
+    return np.packbits(bits, axis=1, bitorder="little").view(np.uint32).view(np.int32).copy()
+
+
+def make(rng, dev, dtype, lanes, per, vocab, history, extra, biases, masked, pad=0):
+    rows = lanes * per
+    import voidinfer_amd as vi
+    wide = torch.from_numpy(rng.standard_normal((rows, vocab + pad)).astype(np.float32) * 3).to(DT_TORCH[dtype]).to(dev)
+    logits = wide[:, :vocab]
+    p = vi.params_array(lanes, repetition_penalty=rng.choice([1.0, 0.9, 1.2, 1.7], lanes),
+                        presence_penalty=rng.choice([0.0, 0.3, -0.2], lanes),
+                        frequency_penalty=rng.choice([0.0, 0.25], lanes))
+    lane_of = np.repeat(np.arange(lanes), per)
+    count = np.zeros((rows, vocab), dtype=np.int64)
+    bias = np.full((rows, vocab), np.nan)
+    allowed = np.ones((rows, vocab), dtype=bool)
+    kw = dict(lanes=torch.from_numpy(lane_of.astype(np.int32)).to(dev))
+
+    def ragged(total, most, low=0):
+        n = rng.integers(low, most + 1, total)
+        return n, np.concatenate([[0], np.cumsum(n)]).astype(np.int64)
+
+    if history:
+        n, off = ragged(lanes, history)
+        h = np.minimum(rng.zipf(1.2, int(off[-1])) - 1, vocab - 1).astype(np.int32)   # repeats many
+        for r, l in enumerate(lane_of):
+            count[r] += np.bincount(h[off[l]:off[l + 1]], minlength=vocab)
+        kw |= dict(histories=torch.from_numpy(h).to(dev), offsets=torch.from_numpy(off).to(dev), max_history=history)
+    if extra:
+        n, off = ragged(rows, extra)
+        e = rng.integers(0, vocab, int(off[-1])).astype(np.int32)
+        for r in range(rows):
+            count[r] += np.bincount(e[off[r]:off[r + 1]], minlength=vocab)
+        kw |= dict(extra=torch.from_numpy(e).to(dev), extra_offsets=torch.from_numpy(off).to(dev))
+    if biases:
+        n, off = ragged(lanes, biases)
+        ids = rng.integers(0, vocab, int(off[-1])).astype(np.int32)   # some twice: the last counts
+        val = rng.uniform(-9, 9, ids.size).astype(np.float32)
+        for r, l in enumerate(lane_of):
+            for i in range(off[l], off[l + 1]):
+                bias[r, ids[i]] = float(val[i])
+        kw |= dict(bias_ids=torch.from_numpy(ids).to(dev), bias_values=torch.from_numpy(val).to(dev),
+                   bias_offsets=torch.from_numpy(off).to(dev))
+    if masked:
+        m = rng.random((max(1, rows // 2), vocab)) < rng.choice([0.98, 0.5, 0.01], (max(1, rows // 2), 1))
+        m[0] = False                                                  # one mask leaves nothing
+        idx = rng.integers(-1, m.shape[0], rows)
+        idx[0] = 0
+        for r in range(rows):
+            if idx[r] >= 0:
+                allowed[r] = m[idx[r]]
+        kw |= dict(masks=torch.from_numpy(pack(m)).to(dev), mask_index=torch.from_numpy(idx.astype(np.int32)).to(dev))
+    return logits, p, lane_of, count, bias, allowed, kw
+
+
+def check(got, logits, dtype, p, lane_of, count, bias, allowed):
+    x = logits.double().cpu().numpy()
+    want, big = reference(x, p, lane_of, count, bias, allowed)
+    g = got.double().cpu().numpy()
+    assert np.array_equal(np.isneginf(g), np.isneginf(want))
+    touched = (count > 0) | ~np.isnan(bias)
+    same = allowed & ~touched
+    assert np.array_equal(g[same], x[same])
+    t = allowed & touched
+    bound = 5 * 2.0 ** -24 * big + UNIT[dtype] * (np.abs(want) + 5 * 2.0 ** -24 * big) + TINY[dtype]
+    assert (np.abs(g[t] - want[t]) <= bound[t]).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("lanes,per,vocab,history,extra,biases,masked,pad", [
+    (1, 1, 1, 3, 0, 1, True, 0),            # one token
+    (1, 1, 31, 5, 2, 2, True, 0),
+    (3, 1, 8192, 50, 0, 0, False, 0),       # one whole slice, penalties alone
+    (2, 3, 8193, 900, 6, 40, True, 3),      # one token past a slice, padded rows
+    (5, 1, 1000, 0, 0, 30, False, 8),       # biases alone
+    (4, 1, 20000, 0, 0, 0, True, 0),        # masks alone
+    (2, 5, 32771, 6000, 16, 300, True, 5),  # everything, odd
+    (1, 4, 151936, 300, 3, 300, True, 0),
+])
+def test_against_the_definition(dev, rng, dtype, lanes, per, vocab, history, extra, biases, masked, pad):
+    import voidinfer_amd as vi
+    case = make(rng, dev, dtype, lanes, per, vocab, history, extra, biases, masked, pad)
+    logits, p, lane_of, count, bias, allowed, kw = case
+    before = logits.clone()
+    print(f"logits dtype {dtype} {lanes}x{per} vocab {vocab}", flush=True)
+    flags = torch.full((lanes * per,), 77, dtype=torch.int32, device=dev)
+    got = vi.process_logits(logits, p, flags=flags, **kw)
+    assert torch.equal(before, logits) and not flags.any()
+    check(got, logits, dtype, p, lane_of, count, bias, allowed)
+    # in place: the same bits, and nothing past the rows' end
+    base = logits._base if logits._base is not None else None
+    tail = None if base is None else base[:, vocab:].clone()
+    vi.process_logits(logits, p, out=logits, **kw)
+    assert torch.equal(got.view(torch.int16 if dtype < 2 else torch.int32),
+                       logits.contiguous().view(torch.int16 if dtype < 2 else torch.int32))
+    if tail is not None:
+        assert torch.equal(base[:, vocab:], tail)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_nonfinite_and_lowest_values(dev, dtype):
+    """NaN, infinities and the type's lowest value where nothing touches them, where a mask hides them and
+    where a penalty or a bias meets them."""
+    import voidinfer_amd as vi
+    lowest = torch.finfo(DT_TORCH[dtype]).min
+    row = [float("nan"), float("inf"), float("-inf"), lowest, -0.0, 1.0, 2.0, 3.0, float("nan"), float("inf")]
+    x = torch.tensor([row, row], dtype=DT_TORCH[dtype], device=dev)
+    p = vi.params_array(2, repetition_penalty=2.0)
+    hist = torch.tensor([0, 1, 2, 3, 4, 0, 1, 2, 3, 4], dtype=torch.int32, device=dev)
+    mask = torch.tensor([[0b0011111111]], dtype=torch.int32, device=dev)
+    out = vi.process_logits(x, p, histories=hist, offsets=torch.tensor([0, 5, 10], device=dev),
+                            bias_ids=torch.tensor([2, 5], dtype=torch.int32, device=dev),
+                            bias_values=torch.tensor([5.0, -1.0], device=dev),
+                            bias_offsets=torch.tensor([0, 2, 2], device=dev), masks=mask,
+                            mask_index=torch.tensor([0, -1], dtype=torch.int32, device=dev)).float().cpu().numpy()
+    a, b = out
+    assert np.isnan(a[0]) and a[1] == np.inf and a[2] == -np.inf and a[3] == -np.inf and a[4] == 0 and a[5] == 0
+    assert a[6] == 2 and a[7] == 3 and a[8] == -np.inf and a[9] == -np.inf      # masked NaN and Inf
+    assert np.isnan(b[0]) and b[5] == 1 and np.isnan(b[8]) and b[9] == np.inf
+
+
+def test_rows_that_cannot_be_done(dev, rng):
+    """A lane out of range, a mask out of range: -Inf throughout and VI_FLAG_ERROR; bad tokens are ignored and
+    flagged; the sampler then reports the row empty."""
+    import voidinfer_amd as vi
+    x = torch.from_numpy(rng.standard_normal((6, 9000)).astype(np.float32)).to(dev).to(torch.bfloat16)
+    p = vi.params_array(3, presence_penalty=1.0)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    flags = i32([0] * 6)
+    out = vi.process_logits(
+        x, p, lanes=i32([0, 3, -1, 1, 2, 2]), histories=i32([5, 9000, -1, 6, 7]),
+        offsets=torch.tensor([0, 3, 3, 5], device=dev), masks=i32([[-1] * 282]), mask_index=i32([0, 0, 0, 1, -5, 0]),
+        flags=flags)
+    assert flags.tolist() == [FLAG_BAD_HISTORY, FLAG_ERROR, FLAG_ERROR, FLAG_ERROR, 0, 0]
+    assert all(torch.isneginf(out[r]).all() for r in (1, 2, 3))
+    want = x.clone()
+    want[0, 5] = (x[0, 5].float() - 1).to(torch.bfloat16)
+    for r in (4, 5):
+        want[r, 6:8] = (x[r, 6:8].float() - 1).to(torch.bfloat16)
+    assert all(torch.equal(out[r], want[r]) for r in (0, 4, 5))
+    s = vi.sample_rows(out, vi.params_array(6))
+    assert [bool(f & vi.FLAG_EMPTY) for f in vi.stats_numpy(s.stats)["flags"]] == [False, True, True, True, False, False]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_same_penalties_as_the_sampler(dev, rng, dtype):
+    """Without biases or masks the rewritten logits are what the sampler works on itself: sampling from
+    them without penalties gives the tokens and uniforms of sampling with them; a penalty state gives the
+    bits that its history gives."""
+    import voidinfer_amd as vi
+    rows, vocab, n = 6, 50_021, 3000
+    x = torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32) * 2).to(DT_TORCH[dtype]).to(dev)
+    fields = dict(seed=rng.integers(1, 2 ** 62, rows), position=rng.integers(0, 10 ** 5, rows), temperature=0.8,
+                  top_p=0.9, top_k=np.array([0, 20, 0, 50, 0, 1]))
+    pen = dict(repetition_penalty=rng.uniform(0.9, 1.5, rows), presence_penalty=rng.uniform(-0.5, 1, rows),
+               frequency_penalty=rng.uniform(0, 0.5, rows))
+    p = vi.params_array(rows, **fields, **pen)
+    hist = torch.from_numpy((rng.zipf(1.3, rows * n) % vocab).astype(np.int32)).to(dev)
+    off = torch.arange(rows + 1, device=dev) * n
+    a = vi.sample_rows(x, p, hist, off, max_history=n)
+    y = vi.process_logits(x, p, histories=hist, offsets=off)
+    b = vi.sample_rows(y, vi.params_array(rows, **fields))
+    assert torch.equal(a.tokens, b.tokens) and torch.equal(a.uniforms, b.uniforms)
+    state = vi.PenaltyState(rows, vocab, 4096, device=dev)
+    state.update(hist, off)
+    z = vi.process_logits(x, p, state=state)
+    as_int = torch.int16 if dtype < 2 else torch.int32
+    assert torch.equal(y.view(as_int), z.view(as_int))
+    # with extra tokens: the state plus them is the history plus them
+    extra = torch.from_numpy(rng.integers(0, vocab, 4 * rows).astype(np.int32)).to(dev)
+    eo = torch.arange(rows + 1, device=dev) * 4
+    both = torch.cat([hist.view(rows, n), extra.view(rows, 4)], 1).reshape(-1)
+    u = vi.process_logits(x, p, state=state, extra=extra, extra_offsets=eo)
+    w = vi.process_logits(x, p, histories=both, offsets=torch.arange(rows + 1, device=dev) * (n + 4))
+    assert torch.equal(u.view(as_int), w.view(as_int))
+
+
+def test_failed_state_and_stream_and_graph(dev, rng):
+    """A penalty state in error fails its row; the call runs on the caller's stream and replays from a graph."""
+    import voidinfer_amd as vi
+    x = torch.from_numpy(rng.standard_normal((2, 20_000)).astype(np.float32)).to(dev).to(torch.float16)
+    p = vi.params_array(2, presence_penalty=1.0)
+    state = vi.PenaltyState(2, 20_000, 64, device=dev)
+    state.update(torch.tensor([3], dtype=torch.int32, device=dev), torch.tensor([0, 1, 1], device=dev), sign=-1)
+    flags = torch.zeros(2, dtype=torch.int32, device=dev)
+    y = vi.process_logits(x, p, state=state, flags=flags)
+    assert flags.tolist() == [FLAG_ERROR, 0] and torch.isneginf(y[0]).all() and torch.equal(y[1], x[1])
+    kw = dict(bias_ids=torch.tensor([1, 19_999], dtype=torch.int32, device=dev),
+              bias_values=torch.tensor([2.0, 3.0], device=dev), bias_offsets=torch.tensor([0, 1, 2], device=dev))
+    p_dev = vi.to_device_bytes(p, dev)
+    want = vi.process_logits(x, p_dev, **kw)
+    out = torch.empty_like(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        vi.process_logits(x, p_dev, out=out, **kw)
+    s.synchronize()
+    assert torch.equal(out, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        vi.process_logits(x, p_dev, out=out, **kw)
+    for _ in range(3):
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_refusals_on_the_device_side(dev):
+    import voidinfer_amd as vi
+    x = torch.zeros(2, 100, dtype=torch.bfloat16, device=dev)
+    i32 = torch.zeros(2, dtype=torch.int32, device=dev)
+    off = torch.zeros(3, dtype=torch.int64, device=dev)
+    for kw in (dict(out=torch.zeros(2, 100, device=dev)), dict(out=x[:1]), dict(lanes=i32.long()), dict(histories=i32),
+               dict(extra=i32), dict(bias_ids=i32, bias_offsets=off), dict(mask_index=i32), dict(flags=i32[:1]),
+               dict(masks=torch.zeros(1, 3, dtype=torch.int32, device=dev), mask_index=i32),
+               dict(masks=torch.zeros(1, 4, dtype=torch.int32, device=dev)),
+               dict(histories=i32, offsets=off[:2], params=vi.params_array(2))):
+        with pytest.raises(ValueError):
+            vi.process_logits(x, **kw)

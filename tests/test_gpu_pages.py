@@ -1,0 +1,321 @@
+"""The page calls against a sequential restatement in Python: whole numbers and
+page contents are equal, entry by entry."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FLAG_ERROR = -(1 << 31)
+
+
+class Model:
+    """refs, tables, lengths and a pool of page contents, one call at a time."""
+
+    def __init__(self, lanes, width, pages, page_size, planes, heads, dim, rng, dtype=torch.bfloat16):
+        self.ps, self.width = page_size, width
+        self.refs = np.zeros(pages, dtype=np.int32)
+        self.tables = np.full((lanes, width), -1, dtype=np.int32)
+        self.lengths = np.zeros(lanes, dtype=np.int32)
+        self.status = np.zeros(3, dtype=np.int32)
+        self.pool = torch.from_numpy(rng.standard_normal((planes, pages, heads, page_size, dim)).astype(np.float32)).to(dtype)
+
+    def held(self, n):
+        return -(-n // self.ps)
+
+    def fork(self, parents, children):
+        good = [(p, c) for i, (p, c) in enumerate(zip(parents, children))
+                if 0 <= p < len(self.lengths) and 0 <= c < len(self.lengths) and c not in parents and
+                children.count(c) == 1 and p not in children]
+        if len(good) < len(parents):
+            self.status[0] = FLAG_ERROR
+        for p, c in good:
+            for page in self.tables[c][self.tables[c] >= 0]:
+                self.refs[page] -= 1
+            self.tables[c] = self.tables[p]
+            for page in self.tables[c][self.tables[c] >= 0]:
+                self.refs[page] += 1
+            self.lengths[c] = self.lengths[p]
+
+    def extend(self, lanes, lengths):
+        bad = len(set(lanes)) < len(lanes) or any(not 0 <= l < len(self.lengths) for l in lanes)
+        bad = bad or any(n < self.lengths[l] or self.held(n) > self.width for l, n in zip(lanes, lengths))
+        refs, tables, pool, taken, copied = self.refs.copy(), self.tables.copy(), self.pool.clone(), 0, 0
+        source = self.pool.clone()
+        pending = np.zeros_like(refs)   # pages given back in this call are free only after it
+        if not bad:
+            try:
+                free = iter(np.flatnonzero(refs == 0).tolist())
+                for l, n in zip(lanes, lengths):
+                    now, e = int(self.lengths[l]), self.held(int(self.lengths[l]))
+                    if now % self.ps and n > now and refs[tables[l, e - 1]] - pending[tables[l, e - 1]] > 1:
+                        old, page = tables[l, e - 1], next(free)
+                        pool[:, page] = source[:, old]
+                        pending[old] += 1
+                        tables[l, e - 1] = page
+                        refs[page] = 1
+                        taken, copied = taken + 1, copied + 1
+                    while e < self.held(n):
+                        tables[l, e] = next(free)
+                        refs[tables[l, e]] = 1
+                        e, taken = e + 1, taken + 1
+            except StopIteration:
+                bad = True
+        if bad:
+            self.status[:] = [FLAG_ERROR, 0, 0]
+            return
+        self.refs, self.tables, self.pool = refs - pending, tables, pool
+        self.lengths[lanes] = lengths
+        self.status[1:] = [taken, copied]
+
+    def truncate(self, lanes, lengths):
+        for l, n in zip(lanes, lengths):
+            if not 0 <= l < len(self.lengths) or n < 0:
+                self.status[0] = FLAG_ERROR
+            elif n < self.lengths[l]:
+                gone = self.tables[l, self.held(n):]
+                np.subtract.at(self.refs, gone[gone >= 0], 1)
+                gone[:] = -1
+                self.lengths[l] = n
+
+    def compact(self):
+        live = int((self.refs > 0).sum())
+        holes = [p for p in range(live) if self.refs[p] == 0]
+        movers = [p for p in range(live, len(self.refs)) if self.refs[p] > 0]
+        for s, t in zip(movers, holes):
+            self.pool[:, t] = self.pool[:, s]
+            self.tables[self.tables == s] = t
+            self.refs[t], self.refs[s] = self.refs[s], 0
+        self.status[1:] = [live, len(movers)]
+
+    def keep(self, lanes, context, paths, kept):
+        before = self.pool.clone()
+        for l, c, path, n in zip(lanes, context, paths, kept):
+            for j in range(n):
+                s, t = c + path[j], c + j
+                self.pool[:, self.tables[l, t // self.ps], :, t % self.ps] = \
+                    before[:, self.tables[l, s // self.ps], :, s % self.ps]
+
+
+class Device:
+    def __init__(self, m, dev):
+        self.dev, self.ps = dev, m.ps
+        self.refs, self.tables, self.lengths, self.status = (torch.from_numpy(x.copy()).to(dev) for x in (
+            m.refs, m.tables, m.lengths, m.status))
+        self.pool = m.pool.to(dev)
+
+    def i32(self, v):
+        return torch.tensor(np.asarray(v, dtype=np.int32), device=self.dev)
+
+    def fork(self, parents, children):
+        import voidinfer_amd as vi
+        vi.pages_fork(self.refs, self.tables, self.lengths, self.i32(parents), self.i32(children), self.ps, self.status)
+
+    def extend(self, lanes, lengths):
+        import voidinfer_amd as vi
+        vi.pages_extend(self.refs, self.tables, self.lengths, self.i32(lanes), self.i32(lengths), self.pool, self.status)
+
+    def truncate(self, lanes, lengths):
+        import voidinfer_amd as vi
+        vi.pages_truncate(self.refs, self.tables, self.lengths, self.i32(lanes), self.i32(lengths), self.ps, self.status)
+
+    def compact(self):
+        import voidinfer_amd as vi
+        vi.pages_compact(self.refs, self.tables, self.pool, self.status)
+
+    def keep(self, lanes, context, paths, kept):
+        import voidinfer_amd as vi
+        vi.keep_rows(self.pool, self.tables, self.i32(lanes), self.i32(context), self.i32(paths), self.i32(kept))
+
+
+def same(m, d, what):
+    assert np.array_equal(d.status.cpu().numpy(), m.status), what
+    assert np.array_equal(d.tables.cpu().numpy(), m.tables), what
+    assert np.array_equal(d.refs.cpu().numpy(), m.refs), what
+    assert np.array_equal(d.lengths.cpu().numpy(), m.lengths), what
+    assert torch.equal(d.pool.cpu().view(torch.int16), m.pool.view(torch.int16)), what
+    held = m.tables[m.tables >= 0]
+    assert np.array_equal(np.bincount(held, minlength=len(m.refs)), m.refs), what   # (the model itself adds up)
+
+
+@pytest.mark.parametrize("page_size,planes,heads,dim,dtype", [(16, 2, 1, 8, torch.bfloat16), (16, 3, 2, 64, torch.float16),
+                                                              (64, 2, 2, 16, torch.bfloat16), (256, 1, 1, 8, torch.float16)])
+def test_a_life_of_lanes(dev, rng, page_size, planes, heads, dim, dtype):
+    """Random calls on a small pool: growth by one token and by many, families that share a last page and
+    grow together, alone or not at all, retirement, compaction, accepted paths, refusals for want of pages."""
+    m = Model(12, 9, 60, page_size, planes, heads, dim, rng, dtype)
+    d = Device(m, dev)
+    for step in range(120):
+        lanes = rng.permutation(12)[:rng.integers(1, 13)].tolist()
+        kind = rng.choice(["extend", "extend", "extend", "fork", "fork", "truncate", "compact", "keep"])
+        print(page_size, step, kind, flush=True)
+        if kind == "extend":
+            args = lanes, [int(min(m.lengths[l] + rng.choice([0, 1, 1, 5, page_size, 3 * page_size]), 9 * page_size)) for l in lanes]
+        elif kind == "fork":
+            n = rng.integers(1, 4)
+            args = [int(lanes[0])] * n, rng.permutation([l for l in range(12) if l != lanes[0]])[:n].tolist()
+        elif kind == "truncate":
+            args = lanes, [int(rng.choice([0, m.lengths[l] // 2, m.lengths[l], m.lengths[l] + 1])) for l in lanes]
+        elif kind == "compact":
+            args = ()
+        else:   # rows appended to pages of their own: the ones that lanes share stay as they are
+            lanes = [l for l in lanes if m.lengths[l] and all(m.refs[p] == 1 for p in m.tables[l][m.tables[l] >= 0])]
+            if not lanes:
+                continue
+            context = [int(rng.integers(max(0, m.lengths[l] - 20), m.lengths[l])) for l in lanes]
+            paths = np.zeros((len(lanes), 21), dtype=np.int32)
+            kept = []
+            for i, l in enumerate(lanes):
+                rows = int(m.lengths[l]) - context[i]
+                path = np.sort(rng.permutation(rows)[:rng.integers(1, rows + 1)])
+                paths[i, :len(path)] = path
+                kept.append(len(path))
+            args = lanes, context, paths.tolist(), kept
+        getattr(m, kind)(*args)
+        getattr(d, kind)(*args)
+        same(m, d, (step, kind, args))
+
+
+@pytest.mark.parametrize("sharers,grow,outside", [(5, 5, False), (5, 3, False), (5, 5, True), (1, 1, True), (2, 2, False)])
+def test_a_shared_last_page(dev, rng, sharers, grow, outside):
+    """Of the lanes that share a partly filled page, every growing one copies it but the last, which keeps the
+    page when nobody else holds it; lanes that stop at the page's end only add a page."""
+    m = Model(8, 4, 40, 16, 2, 1, 8, rng)
+    m.extend([0], [21])
+    m.fork([0] * sharers, list(range(1, 1 + sharers)))
+    if not outside:
+        m.truncate([0], [0])
+    d = Device(m, dev)
+    lanes = rng.permutation(np.arange(1, 1 + sharers))[:grow].tolist()
+    for call in ((lanes, [22] * grow), (lanes, [48] * grow)):
+        m.extend(*call)
+        d.extend(*call)
+        same(m, d, call)
+
+
+@pytest.mark.parametrize("pages", [5, 4096, 4097, 20_000])
+def test_extend_over_pool_sizes(dev, rng, pages):
+    """The lowest free pages in list order, also where the free ones are few and far behind; a list as long
+    as the lanes, and one page too few."""
+    lanes = min(4096, pages)
+    m = Model(lanes + 1, 3, pages, 16, 1, 1, 8, rng)
+    m.refs[rng.random(pages) < 0.5] = 7          # held by somebody else
+    free = int((m.refs == 0).sum())
+    d = Device(m, dev)
+    n = min(lanes, free)
+    order = rng.permutation(lanes)[:n].tolist()
+    for call in ((order[: n // 2], [16] * (n // 2)), (order[n // 2:], [9] * (n - n // 2)), ([lanes], [free * 16 + 1])):
+        if not call[0] or len(call[0]) > 4096:
+            continue
+        m.extend(*call)
+        d.extend(*call)
+        for a, b in ((d.status, m.status), (d.tables, m.tables), (d.refs, m.refs), (d.lengths, m.lengths)):
+            assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("calls", [
+    [("extend", [0, 0], [20, 20])], [("extend", [12], [3])], [("extend", [-1], [3])], [("extend", [0], [9 * 16 + 1])],
+    [("extend", [0], [20]), ("extend", [0, 1], [19, 5])], [("fork", [0], [0])], [("fork", [0, 1], [1, 2])],
+    [("fork", [0, 0], [3, 3])], [("fork", [0], [12])], [("fork", [-2, 0], [1, 2])], [("truncate", [12, 0], [0, 0])],
+    [("truncate", [0], [-1])]])
+def test_refused_on_the_device(dev, rng, calls):
+    """Bad lanes and lengths change nothing (of a fork: nothing of that pair) and set the error flag, which stays."""
+    m = Model(12, 9, 60, 16, 2, 1, 8, rng)
+    d = Device(m, dev)
+    for kind, *args in [("extend", [4], [30])] + calls:
+        getattr(m, kind)(*args)
+        getattr(d, kind)(*args)
+        same(m, d, (kind, args))
+    assert m.status[0] == FLAG_ERROR
+    m.extend([5], [1])
+    d.extend([5], [1])
+    same(m, d, "after")
+
+
+def test_copy_pages(dev, rng):
+    import voidinfer_amd as vi
+    pool = torch.from_numpy(rng.standard_normal((3, 2, 50, 2, 16, 8)).astype(np.float32)).to(dev).to(torch.bfloat16)
+    want = pool.clone()
+    order = rng.permutation(50)
+    s, t = order[:20].astype(np.int32), order[20:40].astype(np.int32)
+    want[:, :, t] = pool[:, :, s]
+    s, t = np.concatenate([s, [50, 3, -1]]).astype(np.int32), np.concatenate([t, [4, -1, 5]]).astype(np.int32)
+    vi.pages_copy(pool, torch.from_numpy(s).to(dev), torch.from_numpy(t).to(dev))
+    assert torch.equal(pool, want)
+    vi.pages_copy(pool, torch.zeros(0, dtype=torch.int32, device=dev), torch.zeros(0, dtype=torch.int32, device=dev))
+    assert torch.equal(pool, want)
+
+
+def test_copy_past_32_bits(dev):
+    """A pool whose last pages lie more than 4 GiB behind the first."""
+    import voidinfer_amd as vi
+    pages = 300
+    pool = torch.zeros(1, pages, 16, 256, 2048, dtype=torch.bfloat16, device=dev)   # 16 MiB a page
+    assert pool.numel() * 2 > 1 << 32
+    pool[0, pages - 1] = 3
+    pool[0, 0, 0, 0, :8] = 5
+    vi.pages_copy(pool, torch.tensor([pages - 1, 0], dtype=torch.int32, device=dev),
+                  torch.tensor([1, pages - 2], dtype=torch.int32, device=dev))
+    assert bool((pool[0, 1] == 3).all()) and bool((pool[0, pages - 2] == pool[0, 0]).all())
+    assert pool[0, pages - 2, 0, 0, 0] == 5 and not pool[0, 2].any() and not pool[0, pages - 3].any()
+
+
+def test_paths_that_are_not_so(dev, rng):
+    """Entries that do not ascend, stand before their place or lead outside the lane's pages are skipped; the
+    others move."""
+    m = Model(3, 2, 10, 16, 2, 2, 8, rng)
+    m.extend([0, 1, 2], [20, 20, 32])
+    d = Device(m, dev)
+    before = m.pool.clone()
+    d.keep([0, 1, 2, 5], [10, 12, 8, 0], [[0, 3, 3, 7], [2, 1, 90, 91], [-1, 4, 5, 6], [1, 2, 3, 4]], [4, 4, 9, 4])
+    got = d.pool.cpu()
+    row = lambda p, l, i: p[:, m.tables[l, i // 16], :, i % 16]  # noqa: E731
+    want = before.clone()
+    for l, c, moves in ((0, 10, {1: 3, 3: 7}), (1, 12, {0: 2}), (2, 8, {1: 4, 2: 5, 3: 6})):
+        for j, s in moves.items():
+            want[:, m.tables[l, (c + j) // 16], :, (c + j) % 16] = row(before, l, c + s)
+    assert torch.equal(got, want)
+
+
+def test_a_round_from_a_graph(dev, rng):
+    """extend, keep_rows and truncate recorded once and replayed: each replay is the round that eager calls make."""
+    import voidinfer_amd as vi
+    m = Model(6, 6, 50, 16, 2, 2, 16, rng)
+    lens = [5, 16, 17, 40, 31, 1]
+    m.extend(list(range(6)), lens)
+    d = Device(m, dev)
+    grown, kept = [n + 9 for n in lens], [1, 2, 3, 4, 5, 9]
+    paths = np.array([[0, 3, 4, 5, 6, 7, 8, 8, 8], [0, 2, 3, 4, 5, 6, 7, 8, 8], [0, 1, 5, 6, 7, 8, 8, 8, 8],
+                      [0, 1, 2, 7, 8, 8, 8, 8, 8], [0, 1, 2, 3, 8, 8, 8, 8, 8], [0, 1, 2, 3, 4, 5, 6, 7, 8]])
+    lanes, lens_d, grown_d, paths_d, kept_d = (d.i32(x) for x in (range(6), lens, grown, paths, kept))
+
+    def round_():
+        vi.pages_extend(d.refs, d.tables, d.lengths, lanes, grown_d, d.pool, d.status)
+        vi.keep_rows(d.pool, d.tables, lanes, lens_d, paths_d, kept_d)
+        vi.pages_truncate(d.refs, d.tables, d.lengths, lanes, lens_d, 16)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        round_()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+
+    def model_round():
+        m.extend(list(range(6)), grown)
+        m.keep(range(6), lens, paths.tolist(), kept)
+        m.truncate(list(range(6)), lens)
+
+    model_round()
+    same(m, d, "on a stream of its own")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        round_()
+    for i in range(3):
+        d.pool.add_(1)
+        m.pool.add_(1)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        model_round()
+        same(m, d, i)

@@ -8,6 +8,7 @@ no caller can silently fall back to a CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -57,6 +58,18 @@ class DeviceSampling(C.Structure):
 
 assert C.sizeof(DeviceSampling) == 40
 
+# Host structs of the logit rules and of the paged cache, packed once per call
+# (field order and padding as in the header).
+LOGIT_RULES = struct.Struct("<12Qqiiii")     # vi_logit_rules
+KV_CACHE = struct.Struct("<2Q3qiiiiii")      # vi_kv_cache
+LANE_ROWS = struct.Struct("<3Qqiiii")        # vi_lane_rows
+HEAD_ROWS = struct.Struct("<Qqq")            # vi_head_rows
+ROTATION = struct.Struct("<3Qiiii")          # vi_rotation
+PAGE_MAP = struct.Struct("<4Qqiiii")         # vi_page_map
+PAGE_POOL = struct.Struct("<Qqqii")          # vi_page_pool
+assert (LOGIT_RULES.size, KV_CACHE.size, LANE_ROWS.size, HEAD_ROWS.size, ROTATION.size, PAGE_MAP.size,
+        PAGE_POOL.size) == (120, 64, 48, 24, 40, 56, 32)
+
 _vp, _i, _i64, _u64, _sz, _u32 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_size_t, C.c_uint32
 
 SIGNATURES = {
@@ -99,6 +112,19 @@ SIGNATURES = {
     "vi_verify_workspace_bytes": ([_i, _i, _i], _sz),
     "vi_verify_rows": ([_i, _vp, _i, _i64, _i, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp,
                         _vp, _sz, _vp], _i),
+    "vi_process_logits": ([_vp, _i, _i, _i, _i64, _vp, _vp, _i64, _vp, _vp], _i),
+    "vi_norm_rotate_append": ([_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp, _i64, _i64, _vp, _vp], _i),
+    "vi_prefix_attention_workspace_bytes": ([_i, _i, _i, _i, _i, _i, _i, _i, _i64, _i64], _sz),
+    "vi_prefix_attention": ([_vp, _vp, _i, _vp, C.c_float, _i, _vp, _vp, _i, _i, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
+                             _vp, _sz, _vp], _i),
+    "vi_pages_fork": ([_vp, _vp, _vp, _i, _vp], _i),
+    "vi_pages_extend_workspace_bytes": ([_i], _sz),
+    "vi_pages_extend": ([_vp, _vp, _vp, _vp, _i, _vp, _sz, _vp], _i),
+    "vi_pages_truncate": ([_vp, _vp, _vp, _i, _vp], _i),
+    "vi_pages_copy": ([_vp, _i, _vp, _vp, _i, _vp], _i),
+    "vi_pages_compact_workspace_bytes": ([_i], _sz),
+    "vi_pages_compact": ([_vp, _vp, _vp, _sz, _vp], _i),
+    "vi_keep_rows": ([_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp], _i),
     "vi_probe_read": ([_vp, _sz, _vp, _vp], _i),
     "vi_probe_copy": ([_vp, _vp, _sz, _vp], _i),
 }

@@ -16,6 +16,36 @@ namespace {
 inline hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 inline bool dtype_ok(int d) { return d == VI_BF16 || d == VI_F16 || d == VI_F32; }
 
+inline bool page_size_ok(int p) { return p >= 16 && p <= 256 && (p & (p - 1)) == 0; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Strides (elements) of 16-byte rows.
+inline bool stride8(int64_t s) { return s >= 0 && s % 8 == 0; }
+
+vi_status cache_ok(const vi_kv_cache* c, const vi_lane_rows* l, int heads) {
+    if (!c || !l || !c->keys || !c->values || !aligned16(c->keys) || !aligned16(c->values) || c->pages <= 0 ||
+        !page_size_ok(c->page_size) || c->kv_heads <= 0 || heads <= 0 || heads % c->kv_heads || c->head_dim <= 0 ||
+        !stride8(c->page_stride) || !stride8(c->head_stride) || !stride8(c->token_stride) || !dtype_ok(c->dtype) ||
+        !l->row_offsets || !l->context || !l->tables || l->table_width <= 0 || l->table_stride < l->table_width ||
+        l->lanes <= 0 || l->rows < 0)
+        return VI_ERR_INVALID;
+    return c->dtype == VI_F32 ? VI_ERR_UNSUPPORTED : VI_OK;
+}
+inline bool head_rows_ok(const vi_head_rows* h) {
+    return h && h->data && aligned16(h->data) && stride8(h->row_stride) && stride8(h->head_stride);
+}
+
+constexpr int kLaneListMax = 4096, kPageLanesMax = 65536;
+vi_status map_ok(const vi_page_map* m, int count, bool refs = true, bool lengths = true) {
+    if (!m || (refs && !m->refs) || !m->tables || (lengths && !m->lengths) || m->pages <= 0 || m->lanes <= 0 || m->table_width <= 0 ||
+        m->table_stride < m->table_width || !page_size_ok(m->page_size) || count < 0)
+        return VI_ERR_INVALID;
+    return m->lanes > kPageLanesMax || count > kLaneListMax ? VI_ERR_UNSUPPORTED : VI_OK;
+}
+inline bool pool_ok(const vi_page_pool* p) {
+    return p && p->base && aligned16(p->base) && p->planes > 0 && p->page_bytes > 0 && p->page_bytes % 16 == 0 &&
+           p->plane_stride >= 0 && p->plane_stride % 16 == 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -319,6 +349,126 @@ vi_status vi_verify_rows(int mode, const void* target, int target_dtype, int64_t
     a.terminal = terminal; a.n_terminal = n_terminal; a.accepted = accepted; a.committed = committed;
     a.committed_count = committed_count; a.lane_flags = lane_flags;
     return launch_verify(a, workspace, workspace_bytes, as_stream(stream));
+}
+
+vi_status vi_process_logits(const void* logits, int dtype, int rows, int vocabulary, int64_t row_stride,
+                            const vi_logit_rules* rules, void* out, int64_t out_stride, uint32_t* row_flags,
+                            void* stream) {
+    if (rows == 0) return VI_OK;
+    if (rows < 0 || vocabulary <= 0 || row_stride < vocabulary || out_stride < vocabulary || !dtype_ok(dtype) ||
+        !logits || !out || !rules || (out == logits && out_stride != row_stride))
+        return VI_ERR_INVALID;
+    const vi_logit_rules& r = *rules;
+    if (r.lanes <= 0 || (!r.row_lanes && rows > r.lanes) || (r.histories && r.states) ||
+        (r.histories && !r.history_offsets) || (r.extra && !r.extra_offsets) ||
+        (r.bias_ids && (!r.bias_values || !r.bias_offsets)) || (r.states && !penalty_slots_ok(r.slots)) ||
+        (r.mask_index && (!r.mask_words || r.masks <= 0 || r.mask_stride < (int64_t(vocabulary) + 31) / 32)))
+        return VI_ERR_INVALID;
+    return launch_rules(logits, dtype, rows, vocabulary, row_stride, r, out, out_stride, row_flags,
+                        as_stream(stream));
+}
+
+vi_status vi_norm_rotate_append(const vi_kv_cache* cache, const vi_lane_rows* lanes, int heads,
+                                const vi_head_rows* queries, const vi_head_rows* keys, const vi_head_rows* values,
+                                const void* query_weight, const void* key_weight, float eps,
+                                const vi_rotation* rotation, void* out, int64_t out_row_stride,
+                                int64_t out_head_stride, uint32_t* row_flags, void* stream) {
+    if (const vi_status s = cache_ok(cache, lanes, heads); s != VI_OK) return s;
+    if (lanes->rows == 0) return VI_OK;
+    if (!head_rows_ok(queries) || !head_rows_ok(keys) || !head_rows_ok(values) || !aligned16(query_weight) ||
+        !aligned16(key_weight) || !rotation || !out || !aligned16(out) || !stride8(out_row_stride) ||
+        !stride8(out_head_stride) || !(eps >= 0.0f) || rotation->rotary_dim < 0 ||
+        rotation->rotary_dim > cache->head_dim ||
+        (rotation->rotary_dim && (!rotation->cosines || !rotation->sines || rotation->angle_rows <= 0)))
+        return VI_ERR_INVALID;
+    if (cache->head_dim % 16 || cache->head_dim > 512 || rotation->rotary_dim % 16) return VI_ERR_UNSUPPORTED;
+    return launch_append(*cache, *lanes, heads, *queries, *keys, *values, query_weight, key_weight, eps, *rotation, out,
+                         out_row_stride, out_head_stride, row_flags, as_stream(stream));
+}
+
+size_t vi_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int lanes, int groups,
+                                           int max_rows, int max_group_rows, int64_t max_own, int64_t max_prefix) {
+    if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || lanes <= 0 || groups < 0 ||
+        max_rows <= 0 || max_group_rows < 0 || max_own < 0 || max_prefix < 0)
+        return 0;
+    return attention_workspace(rows, heads, kv_heads, head_dim, lanes, groups, max_rows, max_group_rows, max_own,
+                               max_prefix);
+}
+
+vi_status vi_prefix_attention(const vi_kv_cache* cache, const vi_lane_rows* lanes, int heads,
+                              const vi_head_rows* queries, float scale, int groups, const int32_t* group_offsets,
+                              const int32_t* prefix_lens, int max_rows, int max_group_rows, int64_t max_own,
+                              int64_t max_prefix, const uint64_t* tree, void* out, int64_t out_row_stride,
+                              int64_t out_head_stride, float* lse, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    if (const vi_status s = cache_ok(cache, lanes, heads); s != VI_OK) return s;
+    if (lanes->rows == 0) return VI_OK;
+    if (!head_rows_ok(queries) || !out || !aligned16(out) || !stride8(out_row_stride) || !stride8(out_head_stride) ||
+        groups < 0 || groups > lanes->lanes || (groups && (!group_offsets || !prefix_lens)) || max_rows <= 0 ||
+        max_own < 0 || max_prefix < 0 || (groups && max_group_rows <= 0) || !(scale == scale))
+        return VI_ERR_INVALID;
+    if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256) return VI_ERR_UNSUPPORTED;
+    return launch_attention(*cache, *lanes, heads, *queries, scale, groups, group_offsets, prefix_lens, max_rows,
+                            max_group_rows, max_own, max_prefix, tree, out, out_row_stride, out_head_stride, lse,
+                            workspace, workspace_bytes, as_stream(stream));
+}
+
+vi_status vi_pages_fork(const vi_page_map* map, const int32_t* parents, const int32_t* children, int count,
+                        void* stream) {
+    if (const vi_status s = map_ok(map, count); s != VI_OK) return s;
+    if (count == 0) return VI_OK;
+    if (!parents || !children) return VI_ERR_INVALID;
+    return launch_pages_fork(*map, parents, children, count, as_stream(stream));
+}
+
+size_t vi_pages_extend_workspace_bytes(int count) { return count <= 0 ? 0 : pages_extend_workspace(count); }
+
+vi_status vi_pages_extend(const vi_page_map* map, const vi_page_pool* pool, const int32_t* lane_ids,
+                          const int32_t* new_lengths, int count, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+    if (const vi_status s = map_ok(map, count); s != VI_OK) return s;
+    if (count == 0) return VI_OK;
+    if (!pool_ok(pool) || !lane_ids || !new_lengths) return VI_ERR_INVALID;
+    return launch_pages_extend(*map, *pool, lane_ids, new_lengths, count, workspace, workspace_bytes,
+                               as_stream(stream));
+}
+
+vi_status vi_pages_truncate(const vi_page_map* map, const int32_t* lane_ids, const int32_t* new_lengths, int count,
+                            void* stream) {
+    if (const vi_status s = map_ok(map, count); s != VI_OK) return s;
+    if (count == 0) return VI_OK;
+    if (!lane_ids || !new_lengths) return VI_ERR_INVALID;
+    return launch_pages_truncate(*map, lane_ids, new_lengths, count, as_stream(stream));
+}
+
+vi_status vi_pages_copy(const vi_page_pool* pool, int pages, const int32_t* sources, const int32_t* targets,
+                        int count, void* stream) {
+    if (!pool_ok(pool) || pages <= 0 || count < 0) return VI_ERR_INVALID;
+    if (count == 0) return VI_OK;
+    if (!sources || !targets) return VI_ERR_INVALID;
+    return launch_pages_copy(*pool, pages, sources, targets, count, as_stream(stream));
+}
+
+size_t vi_pages_compact_workspace_bytes(int pages) { return pages <= 0 ? 0 : pages_compact_workspace(pages); }
+
+vi_status vi_pages_compact(const vi_page_map* map, const vi_page_pool* pool, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+    if (const vi_status s = map_ok(map, 0, true, false); s != VI_OK) return s;
+    if (!pool_ok(pool)) return VI_ERR_INVALID;
+    return launch_pages_compact(*map, *pool, workspace, workspace_bytes, as_stream(stream));
+}
+
+vi_status vi_keep_rows(const vi_page_map* map, const vi_page_pool* pool, int kv_heads, const int32_t* lane_ids,
+                       const int32_t* context, const int32_t* paths, int path_stride, const int32_t* kept,
+                       int count, void* stream) {
+    if (const vi_status s = map_ok(map, count, false, false); s != VI_OK) return s;
+    if (!pool_ok(pool) || kv_heads <= 0 || path_stride <= 0 ||
+        pool->page_bytes % (int64_t(kv_heads) * map->page_size * 16))
+        return VI_ERR_INVALID;
+    if (count == 0) return VI_OK;
+    if (!lane_ids || !context || !paths || !kept) return VI_ERR_INVALID;
+    return launch_keep_rows(*map, *pool, kv_heads, lane_ids, context, paths, path_stride, kept, count,
+                            as_stream(stream));
 }
 
 vi_status vi_probe_read(const void* src, size_t bytes, uint32_t* sink, void* stream) {

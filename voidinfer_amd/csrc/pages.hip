@@ -1,0 +1,460 @@
+// pages.hip — who holds which page of a paged cache (fork, extend, truncate,
+// compact), and the page contents that these move (vi_pages_*, vi_keep_rows).
+//
+// The integers are small and their decisions depend on one another (the lowest
+// free pages go to the lanes in list order), so one workgroup takes each plan:
+// prefix sums over the list and over the reference counts, no atomics whose
+// order could show.  The contents are large and independent: a second launch of
+// many workgroups copies them, reading the planned pairs from device memory, so
+// nothing waits for the host.
+#include <algorithm>
+
+#include "vi_device.h"
+#include "vi_internal.h"
+
+namespace vi {
+namespace {
+
+constexpr int kPlan = 1024;              // threads of a planning workgroup
+constexpr int kListMax = 4096;           // entries of a lane list
+constexpr int kListPer = kListMax / kPlan;
+constexpr int kLanesMax = 65536;
+
+__device__ __forceinline__ int pages_for(int tokens, int page_size) { return (tokens + page_size - 1) / page_size; }
+
+// ---- contents -------------------------------------------------------------------
+struct CopyArgs {
+    vi_page_pool pool;
+    const int32_t* sources;
+    const int32_t* targets;
+    const uint32_t* device_count;   // planned pairs, or NULL: `count`
+    int count, pages;
+};
+
+// Workgroups share out the (pair, plane) blocks.
+__device__ void copy_pages(const CopyArgs& a, unsigned block, unsigned blocks) {
+    const int n = a.device_count ? int(*a.device_count) : a.count;
+    const int64_t items = int64_t(n) * a.pool.planes;
+    const int64_t vecs = a.pool.page_bytes / 16;
+    for (int64_t it = block; it < items; it += blocks) {
+        const int pair = int(it / a.pool.planes), plane = int(it % a.pool.planes);
+        const int s = a.sources[pair], t = a.targets[pair];
+        if (uint32_t(s) >= uint32_t(a.pages) || uint32_t(t) >= uint32_t(a.pages)) continue;
+        unsigned char* const base = static_cast<unsigned char*>(a.pool.base) + int64_t(plane) * a.pool.plane_stride;
+        const uint4* const src = reinterpret_cast<const uint4*>(base + int64_t(s) * a.pool.page_bytes);
+        uint4* const dst = reinterpret_cast<uint4*>(base + int64_t(t) * a.pool.page_bytes);
+        for (int64_t i = threadIdx.x; i < vecs; i += blockDim.x) dst[i] = src[i];
+    }
+}
+
+__global__ __launch_bounds__(256) void copy_kernel(CopyArgs a) { copy_pages(a, blockIdx.x, gridDim.x); }
+
+vi_status launch_copy(const CopyArgs& a, int most, hipStream_t stream) {
+    const int64_t items = int64_t(most) * a.pool.planes;
+    const unsigned blocks = unsigned(std::min<int64_t>(items, 8 * int64_t(device_cus())));
+    hipLaunchKernelGGL(copy_kernel, dim3(blocks), dim3(256), 0, stream, a);
+    return launch_status();
+}
+
+// ---- fork -----------------------------------------------------------------------
+__device__ __forceinline__ void flag_error(int32_t* status) {
+    if (status) atomicOr(reinterpret_cast<uint32_t*>(status), uint32_t(VI_FLAG_ERROR));
+}
+
+__global__ __launch_bounds__(256) void fork_kernel(vi_page_map m, const int32_t* parents, const int32_t* children,
+                                                   int count) {
+    const int i = blockIdx.x, parent = parents[i], child = children[i];
+    bool bad = uint32_t(parent) >= uint32_t(m.lanes) || uint32_t(child) >= uint32_t(m.lanes);
+    for (int j = threadIdx.x; j < count; j += 256) bad |= parents[j] == child || (j != i && children[j] == child);
+    // (a parent that is another pair's child)
+    for (int j = threadIdx.x; j < count; j += 256) bad |= children[j] == parent;
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) flag_error(m.status);
+        return;
+    }
+    const int32_t* const from = m.tables + int64_t(parent) * m.table_stride;
+    int32_t* const to = m.tables + int64_t(child) * m.table_stride;
+    const int length = m.lengths[parent];
+    const int held = min(pages_for(length, m.page_size), m.table_width);
+    for (int e = threadIdx.x; e < m.table_width; e += 256) {
+        const int old = to[e], page = e < held ? from[e] : -1;
+        if (old == page) continue;
+        // (refs only ever count: no page is taken in this launch, so a count that
+        // passes through zero on the way is nobody's to take)
+        if (uint32_t(old) < uint32_t(m.pages)) atomicSub(&m.refs[old], 1);
+        if (uint32_t(page) < uint32_t(m.pages)) atomicAdd(&m.refs[page], 1);
+        to[e] = page;
+    }
+    if (threadIdx.x == 0) m.lengths[child] = length;
+}
+
+// ---- truncate ---------------------------------------------------------------------
+__global__ __launch_bounds__(256) void truncate_kernel(vi_page_map m, const int32_t* lane_ids,
+                                                       const int32_t* new_lengths) {
+    const int lane = lane_ids[blockIdx.x], length = new_lengths[blockIdx.x];
+    if (uint32_t(lane) >= uint32_t(m.lanes) || length < 0) {
+        if (threadIdx.x == 0) flag_error(m.status);
+        return;
+    }
+    const int now = m.lengths[lane];
+    if (length >= now) return;
+    __syncthreads();   // every thread has read the length before it changes
+    int32_t* const table = m.tables + int64_t(lane) * m.table_stride;
+    const int held = min(pages_for(now, m.page_size), m.table_width);
+    for (int e = pages_for(length, m.page_size) + threadIdx.x; e < held; e += 256) {
+        const int page = atomicExch(&table[e], -1);   // (given back once, however often the lane is listed)
+        if (uint32_t(page) < uint32_t(m.pages)) atomicSub(&m.refs[page], 1);
+    }
+    if (threadIdx.x == 0) m.lengths[lane] = length;
+}
+
+// ---- extend -----------------------------------------------------------------------
+struct ExtendWs {
+    uint32_t* pairs;      // planned copies
+    int32_t* sources;
+    int32_t* targets;
+};
+constexpr int kShareSlots = 2 * kListMax;
+
+__global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int32_t* lane_ids,
+                                                       const int32_t* new_lengths, int count, ExtendWs w) {
+    // LDS: which lanes are listed; of the shared last pages, how many listed lanes
+    // hold each and the last of these; the lanes' first new page in rank order
+    __shared__ uint32_t listed[kLanesMax / 32];
+    __shared__ uint32_t keys[kShareSlots];
+    __shared__ uint32_t sharers[kShareSlots];
+    __shared__ uint32_t lasts[kShareSlots];
+    __shared__ uint32_t base[kListMax + 1];
+    __shared__ uint32_t tmp[kPlan / kWave + 1];
+    const int tid = threadIdx.x;
+    int slots = 64;
+    while (slots < 2 * count) slots <<= 1;
+    const int shift = 32 - __builtin_ctz(unsigned(slots));
+    for (int i = tid; i < (m.lanes + 31) / 32; i += kPlan) listed[i] = 0u;
+    for (int i = tid; i < slots; i += kPlan) keys[i] = sharers[i] = lasts[i] = 0u;
+    __syncthreads();
+
+    int lane[kListPer], held[kListPer], need[kListPer], last[kListPer], length[kListPer];
+    uint32_t slot[kListPer];
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < kListPer; ++k) {
+        const int i = tid * kListPer + k;
+        lane[k] = -1; held[k] = need[k] = 0; last[k] = -1; length[k] = 0; slot[k] = 0u;
+        if (i >= count) continue;
+        const int l = lane_ids[i], to = new_lengths[i];
+        if (uint32_t(l) >= uint32_t(m.lanes)) { bad = true; continue; }
+        bad |= (atomicOr(&listed[l >> 5], 1u << (l & 31)) >> (l & 31) & 1u) != 0u;
+        const int now = m.lengths[l], wanted = pages_for(max(to, 0), m.page_size);
+        if (to < now || now < 0 || wanted > m.table_width) { bad = true; continue; }
+        lane[k] = l; length[k] = to;
+        held[k] = pages_for(now, m.page_size);
+        need[k] = wanted - held[k];
+        if (now % m.page_size && to > now) {
+            const int page = m.tables[int64_t(l) * m.table_stride + held[k] - 1];
+            if (uint32_t(page) >= uint32_t(m.pages)) { bad = true; continue; }
+            if (m.refs[page] > 1) {
+                last[k] = page;
+                uint32_t s = (uint32_t(page) * 0x9E3779B1u) >> shift;
+                for (;;) {   // (at most count keys in twice as many slots)
+                    const uint32_t key = atomicCAS(&keys[s], 0u, uint32_t(page) + 1u);
+                    if (key == 0u || key == uint32_t(page) + 1u) break;
+                    s = (s + 1u) & uint32_t(slots - 1);
+                }
+                slot[k] = s;
+                atomicAdd(&sharers[s], 1u);
+                atomicMax(&lasts[s], uint32_t(i));
+            }
+        }
+    }
+    const bool refused = __syncthreads_or(bad);
+    uint32_t mine = 0, copies = 0;
+    bool copied[kListPer];
+#pragma unroll
+    for (int k = 0; k < kListPer; ++k) {
+        const int i = tid * kListPer + k;
+        // the last listed lane keeps the page when the listed ones are all that hold it
+        copied[k] = last[k] >= 0 && !(uint32_t(m.refs[last[k]]) == sharers[slot[k]] && lasts[slot[k]] == uint32_t(i));
+        need[k] += copied[k];
+        mine += uint32_t(need[k]);
+        copies += copied[k];
+    }
+    uint32_t total, pairs;
+    uint32_t at = block_exclusive_scan_u32<kPlan>(mine, tmp, &total);
+    uint32_t pair = block_exclusive_scan_u32<kPlan>(copies, tmp, &pairs);
+    // enough free pages?  (the counts are read again below, from L2)
+    uint32_t free_pages = 0;
+    for (int p0 = 0; p0 < m.pages && free_pages < total; p0 += kPlan * 4) {
+        uint32_t mine_free = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + tid * 4 + j;
+            mine_free += p < m.pages && m.refs[p] == 0;
+        }
+        uint32_t sum;
+        block_exclusive_scan_u32<kPlan>(mine_free, tmp, &sum);
+        free_pages += sum;
+    }
+    if (refused || free_pages < total) {
+        if (tid == 0) {
+            *w.pairs = 0u;
+            if (m.status) { flag_error(m.status); m.status[1] = 0; m.status[2] = 0; }
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < kListPer; ++k) {
+        const int i = tid * kListPer + k;
+        if (i < count) base[i] = at;
+        at += uint32_t(need[k]);
+        if (copied[k]) {   // its copy's target follows below
+            w.sources[pair++] = last[k];
+        }
+    }
+    if (tid == 0) {
+        base[count] = total;
+        *w.pairs = pairs;
+        if (m.status) { m.status[1] = int32_t(total); m.status[2] = int32_t(pairs); }
+    }
+    __syncthreads();
+    // the free pages in ascending order: rank j is the j-th of the list's needs.
+    // Which lane that is and which of its entries: a search in `base`, and what
+    // the lane's thread left in LDS (its held pages, whether the first is a copy).
+    uint32_t* const info = keys;      // [count] held << 1 | copied
+    int32_t* const who = reinterpret_cast<int32_t*>(sharers);
+    uint32_t* const order = lasts;    // [count] the lane's place among the copies
+    __syncthreads();
+    pair -= copies;
+#pragma unroll
+    for (int k = 0; k < kListPer; ++k) {
+        const int i = tid * kListPer + k;
+        if (i >= count) continue;
+        info[i] = uint32_t(held[k]) << 1 | uint32_t(copied[k]);
+        who[i] = lane[k];
+        order[i] = pair;
+        pair += copied[k];
+    }
+    __syncthreads();
+    uint32_t done = 0;
+    for (int p0 = 0; p0 < m.pages && done < total; p0 += kPlan * 4) {
+        uint32_t mine_free = 0;
+        bool is_free[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + tid * 4 + j;
+            is_free[j] = p < m.pages && m.refs[p] == 0;
+            mine_free += is_free[j];
+        }
+        uint32_t sum, rank = done + block_exclusive_scan_u32<kPlan>(mine_free, tmp, &sum);
+        done += sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!is_free[j] || rank >= total) continue;
+            const int p = p0 + tid * 4 + j;
+            int lo = 0, hi = count - 1;   // the last lane whose first rank is not above this one
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (base[mid] <= rank) lo = mid; else hi = mid - 1;
+            }
+            const uint32_t held_l = info[lo] >> 1, copy = info[lo] & 1u, e = rank - base[lo];
+            m.tables[int64_t(who[lo]) * m.table_stride + held_l - copy + e] = p;
+            m.refs[p] = 1;
+            if (copy && e == 0) w.targets[order[lo]] = p;
+            ++rank;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kListPer; ++k) {
+        if (lane[k] < 0) continue;
+        m.lengths[lane[k]] = length[k];
+        if (copied[k]) atomicSub(&m.refs[last[k]], 1);
+    }
+}
+
+// ---- compact ----------------------------------------------------------------------
+struct CompactWs {
+    uint32_t* moved;      // pairs
+    int32_t* sources;     // live pages above the live count, ascending
+    int32_t* targets;     // free pages below it, ascending
+    int32_t* renamed;     // [pages] new id of a page that moves
+};
+
+__global__ __launch_bounds__(kPlan) void compact_kernel(vi_page_map m, CompactWs w) {
+    __shared__ uint32_t tmp[kPlan / kWave + 1];
+    const int tid = threadIdx.x;
+    uint32_t mine = 0, live, scratch;
+    for (int p = tid; p < m.pages; p += kPlan) mine += m.refs[p] != 0;
+    block_exclusive_scan_u32<kPlan>(mine, tmp, &live);
+    uint32_t holes = 0, movers = 0;
+    for (int p0 = 0; p0 < m.pages; p0 += kPlan * 4) {
+        uint32_t h = 0, v = 0;
+        bool hole[4], mover[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + tid * 4 + j;
+            const bool in = p < m.pages, used = in && m.refs[p] != 0;
+            hole[j] = in && !used && uint32_t(p) < live;
+            mover[j] = used && uint32_t(p) >= live;
+            h += hole[j];
+            v += mover[j];
+        }
+        uint32_t nh, nv;
+        uint32_t ah = holes + block_exclusive_scan_u32<kPlan>(h, tmp, &nh);
+        uint32_t av = movers + block_exclusive_scan_u32<kPlan>(v, tmp, &nv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + tid * 4 + j;
+            if (hole[j]) w.targets[ah++] = p;
+            if (mover[j]) w.sources[av++] = p;
+        }
+        holes += nh;
+        movers += nv;
+    }
+    __syncthreads();   // (as many holes as movers: live pages below plus above is the live count)
+    for (uint32_t k = tid; k < movers; k += kPlan) {
+        const int s = w.sources[k], t = w.targets[k];
+        w.renamed[s] = t;
+        m.refs[t] = m.refs[s];
+        m.refs[s] = 0;
+    }
+    if (tid == 0) {
+        *w.moved = movers;
+        if (m.status) { m.status[1] = int32_t(live); m.status[2] = int32_t(movers); }
+    }
+}
+
+// The tables' new ids and the contents in one launch: the first workgroups take
+// the tables.  A page that moved has refs 0 now and one that stayed has not.
+__global__ __launch_bounds__(256) void compact_apply_kernel(vi_page_map m, CopyArgs c, const int32_t* renamed,
+                                                            unsigned table_blocks) {
+    if (blockIdx.x >= table_blocks) {
+        copy_pages(c, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+        return;
+    }
+    const int64_t entries = int64_t(m.lanes) * m.table_width;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < entries; i += int64_t(table_blocks) * 256) {
+        int32_t* const e = m.tables + i / m.table_width * m.table_stride + i % m.table_width;
+        const int p = *e;
+        if (uint32_t(p) < uint32_t(m.pages) && m.refs[p] == 0) *e = renamed[p];
+    }
+}
+
+// ---- accepted rows ------------------------------------------------------------------
+struct KeepArgs {
+    vi_page_map m;
+    vi_page_pool pool;
+    int kv_heads, vecs, path_stride;   // vecs: 16-byte vectors of a token's row in one head
+    const int32_t* lane_ids;
+    const int32_t* context;
+    const int32_t* paths;
+    const int32_t* kept;
+};
+constexpr int kKeepThreads = 256;
+constexpr int kKeepBatch = 4;   // vectors a thread holds between the reads and the writes
+
+// One workgroup per (lane, plane).  Rows move towards the front of an ascending
+// path, so batches in path order never overwrite a row that is still to be
+// read; within a batch every read comes before every write.
+__global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
+    const int i = blockIdx.x / a.pool.planes, plane = blockIdx.x % a.pool.planes, tid = threadIdx.x;
+    const int lane = a.lane_ids[i];
+    if (uint32_t(lane) >= uint32_t(a.m.lanes)) return;
+    const int32_t* const path = a.paths + int64_t(i) * a.path_stride;
+    const int32_t* const table = a.m.tables + int64_t(lane) * a.m.table_stride;
+    const int context = a.context[i], n = min(a.kept[i], a.path_stride), per_row = a.kv_heads * a.vecs;
+    if (context < 0) return;
+    unsigned char* const base = static_cast<unsigned char*>(a.pool.base) + int64_t(plane) * a.pool.plane_stride;
+    auto place = [&](int64_t index, int head, int vec) -> uint4* {
+        const int64_t e = index / a.m.page_size;
+        if (index < 0 || e >= a.m.table_width) return nullptr;
+        const int page = table[e];
+        if (uint32_t(page) >= uint32_t(a.m.pages)) return nullptr;
+        return reinterpret_cast<uint4*>(base + int64_t(page) * a.pool.page_bytes) +
+               (int64_t(head) * a.m.page_size + index % a.m.page_size) * a.vecs + vec;
+    };
+    int j0 = 0;   // rows that stay in place need nothing
+    while (j0 < n && path[j0] == j0) ++j0;
+    const int64_t items = int64_t(n - j0) * per_row;
+    for (int64_t b = 0; b < items; b += kKeepThreads * kKeepBatch) {
+        uint4 v[kKeepBatch];
+        uint4* to[kKeepBatch];
+#pragma unroll
+        for (int k = 0; k < kKeepBatch; ++k) {
+            const int64_t it = b + k * kKeepThreads + tid;
+            to[k] = nullptr;
+            if (it >= items) continue;
+            const int j = j0 + int(it / per_row), head = int(it % per_row) / a.vecs, vec = int(it % a.vecs);
+            const int from = path[j];
+            if (from <= j || from >= 65536 || (j > 0 && path[j - 1] >= from)) continue;
+            const uint4* const src = place(int64_t(context) + from, head, vec);
+            to[k] = place(int64_t(context) + j, head, vec);
+            if (src && to[k]) v[k] = *src; else to[k] = nullptr;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kKeepBatch; ++k)
+            if (to[k]) *to[k] = v[k];
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+vi_status launch_pages_fork(const vi_page_map& m, const int32_t* parents, const int32_t* children, int count,
+                            hipStream_t stream) {
+    hipLaunchKernelGGL(fork_kernel, dim3(count), dim3(256), 0, stream, m, parents, children, count);
+    return launch_status();
+}
+
+vi_status launch_pages_truncate(const vi_page_map& m, const int32_t* lane_ids, const int32_t* new_lengths, int count,
+                                hipStream_t stream) {
+    hipLaunchKernelGGL(truncate_kernel, dim3(count), dim3(256), 0, stream, m, lane_ids, new_lengths);
+    return launch_status();
+}
+
+size_t pages_extend_workspace(int count) { return 256 + 2 * align_up(size_t(count) * 4, 256); }
+
+vi_status launch_pages_extend(const vi_page_map& m, const vi_page_pool& pool, const int32_t* lane_ids,
+                              const int32_t* new_lengths, int count, void* ws, size_t ws_bytes, hipStream_t stream) {
+    Carver c(ws, ws_bytes);
+    ExtendWs w{c.take<uint32_t>(1), c.take<int32_t>(count), c.take<int32_t>(count)};
+    if (!c.ok) return VI_ERR_WORKSPACE;
+    hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(kPlan), 0, stream, m, lane_ids, new_lengths, count, w);
+    if (const vi_status s = launch_status(); s != VI_OK) return s;
+    CopyArgs a{pool, w.sources, w.targets, w.pairs, count, m.pages};
+    return launch_copy(a, count, stream);
+}
+
+vi_status launch_pages_copy(const vi_page_pool& pool, int pages, const int32_t* sources, const int32_t* targets,
+                            int count, hipStream_t stream) {
+    CopyArgs a{pool, sources, targets, nullptr, count, pages};
+    return launch_copy(a, count, stream);
+}
+
+size_t pages_compact_workspace(int pages) { return 256 + 3 * align_up(size_t(pages) * 4, 256); }
+
+vi_status launch_pages_compact(const vi_page_map& m, const vi_page_pool& pool, void* ws, size_t ws_bytes,
+                               hipStream_t stream) {
+    Carver c(ws, ws_bytes);
+    CompactWs w{c.take<uint32_t>(1), c.take<int32_t>(m.pages), c.take<int32_t>(m.pages), c.take<int32_t>(m.pages)};
+    if (!c.ok) return VI_ERR_WORKSPACE;
+    hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kPlan), 0, stream, m, w);
+    if (const vi_status s = launch_status(); s != VI_OK) return s;
+    CopyArgs a{pool, w.sources, w.targets, w.moved, m.pages, m.pages};
+    const int64_t entries = int64_t(m.lanes) * m.table_width;
+    const unsigned tables = unsigned(std::clamp<int64_t>((entries + 1023) / 1024, 1, 64));
+    const unsigned copies = unsigned(std::min<int64_t>(int64_t(m.pages) * pool.planes, 8 * int64_t(device_cus())));
+    hipLaunchKernelGGL(compact_apply_kernel, dim3(tables + copies), dim3(256), 0, stream, m, a, w.renamed, tables);
+    return launch_status();
+}
+
+vi_status launch_keep_rows(const vi_page_map& m, const vi_page_pool& pool, int kv_heads, const int32_t* lane_ids,
+                           const int32_t* context, const int32_t* paths, int path_stride, const int32_t* kept,
+                           int count, hipStream_t stream) {
+    KeepArgs a{m, pool, kv_heads, int(pool.page_bytes / (int64_t(kv_heads) * m.page_size * 16)), path_stride,
+               lane_ids, context, paths, kept};
+    hipLaunchKernelGGL(keep_kernel, dim3(unsigned(count) * pool.planes), dim3(kKeepThreads), 0, stream, a);
+    return launch_status();
+}
+
+}  // namespace vi

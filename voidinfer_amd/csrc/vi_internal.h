@@ -249,6 +249,39 @@ struct VerifyArgs {
 size_t verify_workspace(int lanes, int drafts, int vocabulary);
 vi_status launch_verify(const VerifyArgs& a, void* ws, size_t ws_bytes, hipStream_t stream);
 
+// ---- logit rules (logits.hip) ------------------------------------------------------
+vi_status launch_rules(const void* logits, int dtype, int rows, int vocabulary, int64_t stride,
+                       const vi_logit_rules& rules, void* out, int64_t out_stride, uint32_t* row_flags,
+                       hipStream_t stream);
+
+// ---- paged cache (append.hip, attention.hip, pages.hip) -----------------------------
+vi_status launch_append(const vi_kv_cache& cache, const vi_lane_rows& lanes, int heads, const vi_head_rows& q,
+                        const vi_head_rows& k, const vi_head_rows& v, const void* q_weight, const void* k_weight,
+                        float eps, const vi_rotation& rot, void* out, int64_t out_row, int64_t out_head,
+                        uint32_t* row_flags, hipStream_t stream);
+size_t attention_workspace(int rows, int heads, int kv_heads, int head_dim, int lanes, int groups, int max_rows,
+                           int max_group_rows, int64_t max_own, int64_t max_prefix);
+vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, int heads, const vi_head_rows& q,
+                           float scale, int groups, const int32_t* group_offsets, const int32_t* prefix_lens,
+                           int max_rows, int max_group_rows, int64_t max_own, int64_t max_prefix,
+                           const uint64_t* tree, void* out, int64_t out_row, int64_t out_head, float* lse, void* ws,
+                           size_t ws_bytes, hipStream_t stream);
+vi_status launch_pages_fork(const vi_page_map& m, const int32_t* parents, const int32_t* children, int count,
+                            hipStream_t stream);
+size_t pages_extend_workspace(int count);
+vi_status launch_pages_extend(const vi_page_map& m, const vi_page_pool& pool, const int32_t* lane_ids,
+                              const int32_t* new_lengths, int count, void* ws, size_t ws_bytes, hipStream_t stream);
+vi_status launch_pages_truncate(const vi_page_map& m, const int32_t* lane_ids, const int32_t* new_lengths, int count,
+                                hipStream_t stream);
+vi_status launch_pages_copy(const vi_page_pool& pool, int pages, const int32_t* sources, const int32_t* targets,
+                            int count, hipStream_t stream);
+size_t pages_compact_workspace(int pages);
+vi_status launch_pages_compact(const vi_page_map& m, const vi_page_pool& pool, void* ws, size_t ws_bytes,
+                               hipStream_t stream);
+vi_status launch_keep_rows(const vi_page_map& m, const vi_page_pool& pool, int kv_heads, const int32_t* lane_ids,
+                           const int32_t* context, const int32_t* paths, int path_stride, const int32_t* kept,
+                           int count, hipStream_t stream);
+
 // ---- probes -----------------------------------------------------------------------
 vi_status launch_probe_read(const void* src, size_t bytes, uint32_t* sink, hipStream_t stream);
 vi_status launch_probe_copy(void* dst, const void* src, size_t bytes, hipStream_t stream);

@@ -389,6 +389,89 @@ def sample_rows_state(logits: torch.Tensor, params: np.ndarray | torch.Tensor, s
     return o
 
 
+def _int_list(t: torch.Tensor, dtype: torch.dtype, name: str, count: int | None = None) -> int:
+    """Address of a contiguous 1-d device list of `dtype` (with `count` entries, where that is given)."""
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{name} must be a contiguous 1-d device tensor of {dtype}")
+    if count is not None and t.numel() != count:
+        raise ValueError(f"{name} must have {count} entries")
+    return t.data_ptr()
+
+
+def process_logits(logits: torch.Tensor, params: np.ndarray | torch.Tensor | None = None, *,
+                   lanes: torch.Tensor | None = None, histories: torch.Tensor | None = None,
+                   offsets: torch.Tensor | None = None, state: PenaltyState | None = None,
+                   extra: torch.Tensor | None = None, extra_offsets: torch.Tensor | None = None,
+                   bias_ids: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                   bias_offsets: torch.Tensor | None = None, masks: torch.Tensor | None = None,
+                   mask_index: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                   flags: torch.Tensor | None = None, max_history: int = 0) -> torch.Tensor:
+    """Penalties, biases and grammar masks applied to logits [rows, vocabulary]
+    (vi_process_logits); returns `out` (a new tensor of the logits' type, or the
+    one given: `logits` itself for in place).
+
+    params: vi_row_params per lane (its penalties; host array or device uint8);
+    lanes: int32 [rows], each row's lane (without it row r is lane r); histories
+    int32 with int64 offsets [lanes + 1], or a PenaltyState; extra int32 with
+    int64 extra_offsets [rows + 1], more history per row; bias_ids int32 /
+    bias_values fp32 with int64 bias_offsets [lanes + 1]; masks int32 [n, words]
+    with mask_index int32 [rows] (negative: no mask); flags: int32 [rows], the
+    rows' VI_FLAG_* bits.  `max_history` is not needed (sample_rows' callers
+    have it at hand) and any history length is taken."""
+    dtype, rows, vocab, stride = _logit_args(logits)
+    dev = logits.device
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
+    elif out.dtype != logits.dtype or out.shape != logits.shape or out.stride(1) != 1 or not out.is_cuda:
+        raise ValueError("out must have the logits' shape and type, rows contiguous")
+    out_stride = out.stride(0) if rows > 1 else max(vocab, out.stride(0))
+    p_ptr = n_lanes = 0
+    if params is not None:
+        p_dev = params if isinstance(params, torch.Tensor) else to_device_bytes(params, dev)
+        if p_dev.dtype != torch.uint8 or not p_dev.is_cuda:
+            raise ValueError("params must be vi_row_params (device bytes)")
+        p_ptr, n_lanes = p_dev.data_ptr(), p_dev.numel() // ROW_PARAMS.itemsize
+    lists = (offsets, bias_offsets)
+    n_lanes = n_lanes or next((t.numel() - 1 for t in lists if t is not None), rows)
+    if any(t is not None and t.numel() != n_lanes + 1 for t in lists):
+        raise ValueError("offsets and bias_offsets must have lanes + 1 entries")
+    row_lanes = 0 if lanes is None else _int_list(lanes, torch.int32, "lanes", rows)
+    h = ho = e = eo = bi = bv = bo = m = mi = stride_m = n_masks = st = slots = 0
+    if histories is not None:
+        if offsets is None or state is not None:
+            raise ValueError("histories need offsets and exclude a penalty state")
+        h, ho = _int_list(histories, torch.int32, "histories"), _int_list(offsets, torch.int64, "offsets")
+    if state is not None:
+        if n_lanes > state.lanes or vocab != state.vocabulary:
+            raise ValueError("penalty state has too few lanes or another vocabulary")
+        st, slots = state.buf.data_ptr(), state.slots
+    if extra is not None:
+        if extra_offsets is None:
+            raise ValueError("extra needs extra_offsets")
+        e = _int_list(extra, torch.int32, "extra")
+        eo = _int_list(extra_offsets, torch.int64, "extra_offsets", rows + 1)
+    if bias_ids is not None:
+        if bias_values is None or bias_offsets is None:
+            raise ValueError("bias_ids need bias_values and bias_offsets")
+        bi = _int_list(bias_ids, torch.int32, "bias_ids")
+        bv = _int_list(bias_values, torch.float32, "bias_values", bias_ids.numel())
+        bo = _int_list(bias_offsets, torch.int64, "bias_offsets")
+    if mask_index is not None:
+        if masks is None or masks.dtype != torch.int32 or masks.dim() != 2 or masks.stride(1) != 1 or \
+                masks.shape[1] * 32 < vocab:
+            raise ValueError("masks must be int32 [n, ceil(vocabulary / 32)] with contiguous rows")
+        mi = _int_list(mask_index, torch.int32, "mask_index", rows)
+        m, n_masks, stride_m = masks.data_ptr(), masks.shape[0], max(masks.stride(0), masks.shape[1])
+    elif masks is not None:
+        raise ValueError("masks need mask_index")
+    f = 0 if flags is None else _int_list(flags, torch.int32, "flags", rows)
+    rules = _abi.LOGIT_RULES.pack(p_ptr, row_lanes, h, ho, st, e, eo, bi, bv, bo, m, mi, stride_m, n_lanes, n_masks,
+                                  slots, 0)
+    check(_lib().vi_process_logits(logits.data_ptr(), dtype, rows, vocab, stride, rules, out.data_ptr(), out_stride,
+                                   f, _stream()), "vi_process_logits")
+    return out
+
+
 def stats_numpy(stats: torch.Tensor) -> np.ndarray:
     return stats.cpu().numpy().view(SAMPLE_STATS)
 
