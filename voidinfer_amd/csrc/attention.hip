@@ -1,20 +1,51 @@
-// attention.hip — attention of the lanes' rows over their paged cache
-// (vi_prefix_attention).
+// attention.hip — attention of the lanes' rows over their paged cache, a prefix
+// that the lanes of a group share read once for all of them (vi_prefix_attention).
 //
-// One wave per (row, query head), one pass over the row's keys with a running
-// maximum m and sum l per lane of the wave: each lane takes every 64th key whole
-// and keeps its own m, l and weighted values in LDS, joined at the end.
+// Work: a scope is a set of consecutive rows that see the same keys through one
+// table: a group's rows over its prefix, or a lane's rows over the tokens
+// past it.  Its queries are rows x (heads per kv head), and a workgroup takes up
+// to 128 of them over one chunk of the keys for one kv head, in one pass with a
+// running maximum and sum.  The parts' sums meet in a second launch.
+//
+// The products are transposed: S^T = K Q^T (32 keys x 32 queries a matrix
+// instruction) leaves each lane the scores of one query, so the softmax needs one
+// exchange between the wave's halves, and its weights are already in the layout
+// that O^T = V^T P^T takes as its second operand.  V^T is read from LDS by the
+// transposing loads.  Keys and values arrive in LDS by direct loads, one tile
+// ahead; 16-byte chunks of a row are permuted by the row's number, so that the
+// 16 rows that a fragment read touches at once, and the 4 rows x 64 bytes of a
+// transposing read, fall into different banks.
+#include <algorithm>
+
 #include "cache_rows.h"
 
 namespace vi {
 namespace {
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnWaves = kAttnThreads / kWave;
+constexpr int kPageList = 256;     // pages of a segment of the keys
+constexpr int kTileBytes = 16384;  // a tile's keys (and its values) in LDS
+constexpr float kLog2e = 1.44269504088896340736f;
+// A running maximum is raised (and the sums rescaled) only once a score exceeds
+// it by this many powers of two: weights stay below 2^8, far from fp16's range.
+constexpr float kSlack = 8.0f;
+
+struct ScopePlan {
+    int tiles, waves, splits, chunk;   // query tiles, waves along queries, chunks of the keys, keys a chunk
+};
+struct AttnPlan {
+    ScopePlan prefix, own;
+    int parts() const { return prefix.splits + own.splits; }
+};
 
 struct AttnArgs {
     vi_kv_cache cache;
     vi_lane_rows lanes;
     vi_head_rows q;
     int heads, groups;
-    float scale;
+    float scale2;          // |scale| log2(e)
+    uint32_t flip;         // sign bits of a negative scale, applied to the queries
     const int32_t* group_offsets;
     const int32_t* prefix_lens;
     int max_rows, max_group_rows;
@@ -22,76 +53,552 @@ struct AttnArgs {
     void* out;
     int64_t out_row, out_head;
     float* lse;
+    AttnPlan plan;
+    float* part_o;         // [parts][rows * heads][head_dim], unnormalised
+    float2* part_ml;       // [parts][rows * heads]: maximum (raw scores), sum (negative: marked)
 };
 
-template <int DT>
-__global__ __launch_bounds__(64) void attention_row_kernel(AttnArgs a) {
-    __shared__ float qs[512];
-    __shared__ float acc[512];
-    const int r = blockIdx.x / a.heads, h = blockIdx.x % a.heads, t = threadIdx.x, d = a.cache.head_dim;
-    if (r >= a.lanes.row_offsets[a.lanes.lanes]) return;
-    const int lane = lane_of_row(a.lanes.row_offsets, a.lanes.lanes, r);
-    const int i = r - a.lanes.row_offsets[lane], rows = a.lanes.row_offsets[lane + 1] - a.lanes.row_offsets[lane];
-    const int kv = h / (a.heads / a.cache.kv_heads);
-    const int64_t context = a.lanes.context[lane];
-    int first = lane, prefix = 0, group_rows = 0;
-    for (int g = 0; g < a.groups; ++g)
-        if (a.group_offsets[g] <= lane && lane < a.group_offsets[g + 1]) {
-            first = a.group_offsets[g];
-            prefix = a.prefix_lens[g];
-            group_rows = a.lanes.row_offsets[a.group_offsets[g + 1]] - a.lanes.row_offsets[first];
-        }
-    const uint16_t* const q = static_cast<const uint16_t*>(a.q.data) + int64_t(r) * a.q.row_stride + int64_t(h) * a.q.head_stride;
-    for (int e = t; e < d; e += 64) { qs[e] = Elem<DT>::decode(q[e]) * a.scale; acc[e] = 0.0f; }
-    __syncthreads();
-    const uint64_t seen = a.tree ? a.tree[r] : 0;
-    float m = -kInfF, l = 0.0f;
-    bool poison = i >= a.max_rows || (a.groups && group_rows > a.max_group_rows);
-    for (int64_t k0 = 0; k0 < context + rows; k0 += 64) {
-        const int64_t at = k0 + t, j = at - context;
-        bool see = at < context + rows && (j < 0 || (a.tree ? j < 64 && (seen >> j & 1) : j <= i));
-        float s = -kInfF;
-        const uint16_t* vrow = nullptr;
-        if (see) {
-            const int page = page_of(a.lanes, a.cache.pages, a.cache.page_size, at < prefix ? first : lane, at);
-            if (page < 0) {
-                poison = true;
-            } else {
-                const int64_t o = int64_t(page) * a.cache.page_stride + int64_t(kv) * a.cache.head_stride +
-                                  int64_t(at & (a.cache.page_size - 1)) * a.cache.token_stride;
-                const uint16_t* const krow = static_cast<const uint16_t*>(a.cache.keys) + o;
-                vrow = static_cast<const uint16_t*>(a.cache.values) + o;
-                s = 0.0f;
-                for (int e = 0; e < d; ++e) s = fmaf(qs[e], Elem<DT>::decode(krow[e]), s);
-            }
-        }
-        float top = s;
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
-        const float next = fmaxf(m, top);
-        if (next == -kInfF) continue;
-        const float shrink = expf(m - next), w = vrow ? expf(s - next) : 0.0f;
-        float sum = w;
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-        l = l * shrink + sum;
-        m = next;
-        for (int e = 0; e < d; ++e) {
-            float x = vrow ? w * Elem<DT>::decode(vrow[e]) : 0.0f;
-            for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o, kWave);
-            if (t == 0) acc[e] = acc[e] * shrink + x;
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+template <int DT> __device__ __forceinline__ f32x16_t mfma(s16x8_t a, s16x8_t b, f32x16_t c) {
+    if constexpr (DT == VI_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    }
+}
+template <int DT> __device__ __forceinline__ s16x8_t pack8(const float* p) {
+    if constexpr (DT == VI_BF16) {
+        bf16x8_t r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = static_cast<__bf16>(p[j]);
+        return __builtin_bit_cast(s16x8_t, r);
+    } else {
+        f16x8_t r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = static_cast<_Float16>(p[j]);
+        return __builtin_bit_cast(s16x8_t, r);
+    }
+}
+
+// 16 bytes a lane from its address to LDS (`to`: wave-uniform, lane i's bytes at
+// 16 i), without registers in between.  In assembly because the compiler waits for
+// every such load before any later read of LDS, also of another buffer: the
+// loads of the next tile would not run beside the work on this one.  loads_done()
+// waits for the wave's own, a barrier behind it for everyone's.
+__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(
+        uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to)));
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <class T> __device__ __forceinline__ __attribute__((address_space(3))) T* lds_ptr(uint32_t at) {
+    return (__attribute__((address_space(3))) T*)at;
+}
+
+// A row's chunk c is stored at c ^ swizzle(row).
+template <int D> __device__ __forceinline__ constexpr int swizzle(int row) {
+    return D == 64 ? ((row >> 1 & 1) << 2) | (row >> 2 & 3) : ((row & 3) << 2) | (row >> 2 & 3);
+}
+// All ones where bit b of x is set.
+__device__ __forceinline__ uint32_t bit_mask(uint32_t x, int b) { return uint32_t(int32_t(x << (31 - b)) >> 31); }
+template <int DT> __device__ __forceinline__ s16x8_t finite_or_zero(s16x8_t v) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    constexpr uint32_t kStep = DT == VI_BF16 ? 0x00800080u : 0x04000400u;   // carries out of an exponent of ones
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = ((w[i] & 0x7fff7fffu) + kStep) & 0x80008000u;
+        w[i] &= ~((t >> 15) * 0xffffu);
+    }
+    return __builtin_bit_cast(s16x8_t, w);
+}
+// What sums taken against maximum `from` become against `to` (-Inf: nothing was seen yet; a scale of 0 is one).
+__device__ __forceinline__ float rescale(float from, float to, float scale2) {
+    return from == to ? 1.0f : from == -kInfF ? 0.0f : exp2f((from - to) * scale2);
+}
+// The lowest n bits (none below 0, all from 64 on).
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+// The larger of the two halves' values, in both.
+__device__ __forceinline__ float halves_max(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];   // (a bit cast of a vector's element would take element 0)
+    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// The scope of a row range: its rows, keys and table.
+struct Scope {
+    int row0, rows, table;   // first row, rows, lane whose table is read
+    int64_t begin, end;      // keys
+    int64_t context;         // keys below it are seen by every row
+};
+__device__ __forceinline__ int64_t prefix_of_lane(const AttnArgs& a, int lane) {
+    if (!a.groups) return 0;
+    const int g = lane_of_row(a.group_offsets, a.groups, lane);
+    if (lane < a.group_offsets[g] || lane >= a.group_offsets[g + 1]) return 0;
+    return max(a.prefix_lens[g], 0);
+}
+__device__ __forceinline__ Scope own_scope(const AttnArgs& a, int lane) {
+    Scope s;
+    s.row0 = a.lanes.row_offsets[lane];
+    s.rows = a.lanes.row_offsets[lane + 1] - s.row0;
+    s.table = lane;
+    s.context = max(a.lanes.context[lane], 0);
+    s.begin = min(prefix_of_lane(a, lane), s.context);
+    s.end = s.context + s.rows;
+    return s;
+}
+__device__ __forceinline__ Scope prefix_scope(const AttnArgs& a, int g) {
+    Scope s;
+    const int first = a.group_offsets[g], last = a.group_offsets[g + 1];
+    s.row0 = a.lanes.row_offsets[first];
+    s.rows = last > first ? a.lanes.row_offsets[last] - s.row0 : 0;
+    s.table = first;
+    s.begin = 0;
+    s.end = s.context = max(a.prefix_lens[g], 0);
+    return s;
+}
+// Part `split` of a scope's keys: the last takes what is left.
+__device__ __forceinline__ void part_range(const Scope& s, const ScopePlan& p, int split, int64_t* k0, int64_t* k1) {
+    *k0 = min(s.begin + int64_t(split) * p.chunk, s.end);
+    *k1 = split == p.splits - 1 ? s.end : min(*k0 + p.chunk, s.end);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
+    constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
+    constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
+    constexpr int kLoads = kKeys / kRowsPerLoad / kAttnWaves;           // loads of a wave for a tile's keys
+    constexpr int kSteps = D / 16, kOuts = D / 32;
+    __shared__ __align__(1024) unsigned char tiles[2][2][kTileBytes];   // [stage][keys, values]
+    __shared__ int page_list[kPageList];
+
+    const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int col = lane & 31, half = lane >> 5;
+    const int kv_heads = a.cache.kv_heads, per_kv = a.heads / kv_heads, ps = a.cache.page_size;
+    const int shift = __builtin_ctz(unsigned(ps));
+
+    // which item: heads fastest, so that one head's tiles stay on one XCD's L2 where heads are a multiple of 8
+    const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
+    int item = blockIdx.x;
+    const bool is_prefix = item < prefix_items;
+    if (!is_prefix) item -= prefix_items;
+    const ScopePlan& plan = is_prefix ? a.plan.prefix : a.plan.own;
+    const int head = item % kv_heads;
+    item /= kv_heads;
+    const int tile = item % plan.tiles;
+    item /= plan.tiles;
+    const int split = item % plan.splits, which = item / plan.splits;
+    const Scope s = is_prefix ? prefix_scope(a, which) : own_scope(a, which);
+    const int queries = min(s.rows, is_prefix ? a.max_group_rows : a.max_rows) * per_kv;
+    const int m0 = tile * 32 * plan.waves;
+    int64_t k0, k1;
+    part_range(s, plan, split, &k0, &k1);
+    if (m0 >= queries || k0 >= k1) return;
+
+    // the wave's queries and its blocks of a tile's keys
+    const int along_keys = min(kAttnWaves / plan.waves, kBlocks);
+    const int qi = wave % plan.waves, ki = wave / plan.waves;
+    const int m = m0 + qi * 32 + col;
+    const bool active = m0 + qi * 32 < queries && ki < along_keys;
+    const bool live = active && m < queries;
+    const int row = s.row0 + (live ? m / per_kv : 0), own_row = live ? m / per_kv : 0;
+    const int qhead = head * per_kv + (live ? m % per_kv : 0);
+    s16x8_t qf[kSteps];
+    {
+        const uint16_t* const q = static_cast<const uint16_t*>(a.q.data) + int64_t(row) * a.q.row_stride +
+                                  int64_t(qhead) * a.q.head_stride;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live) v = *reinterpret_cast<const uint4*>(q + k * 16 + half * 8);
+            v.x ^= a.flip; v.y ^= a.flip; v.z ^= a.flip; v.w ^= a.flip;
+            qf[k] = __builtin_bit_cast(s16x8_t, v);
         }
     }
-    if (ballot(poison)) l = m = __builtin_nanf("");
-    __syncthreads();
-    uint16_t* const out = static_cast<uint16_t*>(a.out) + int64_t(r) * a.out_row + int64_t(h) * a.out_head;
-    for (int e = t; e < d; e += 64) out[e] = uint16_t(Elem<DT>::round(l == 0.0f ? 0.0f : acc[e] / l));
-    if (a.lse && t == 0) a.lse[int64_t(r) * a.heads + h] = l == 0.0f ? -kInfF : m + logf(l);
+    const uint64_t seen = live && a.tree && !is_prefix ? a.tree[row] : 0;
+
+    const uint32_t tile_at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&tiles));
+    // keys: lane (col, half) reads chunk 2 k + half of row col; values: lane i of 16 reads 4 of the
+    // 16 places of row i / 4 (rows 4 half .. 4 half + 3, and the same 8 rows on)
+    const int sub = lane & 15, value_row = 4 * half + sub / 4;
+    const uint32_t key_lane = uint32_t(col * 2 * D + ((half ^ swizzle<D>(col)) << 4));
+    const uint32_t value_lane =
+        uint32_t(value_row * 2 * D + (((2 * (lane >> 4 & 1) + (sub >> 1 & 1)) ^ swizzle<D>(value_row)) << 4) + (sub & 1) * 8);
+    constexpr uint32_t kValueFlip = uint32_t(swizzle<D>(8)) << 4;   // (swizzle is linear in the row's bits)
+
+    f32x16_t acc[kOuts];
+#pragma unroll
+    for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+    float top = -kInfF, sum = 0.0f;   // raw score units; this half's sum
+    bool marked = false;
+
+    const int32_t* const table = a.lanes.tables + int64_t(s.table) * a.lanes.table_stride;
+    const int64_t head_offset = int64_t(head) * a.cache.head_stride;
+
+    for (int64_t seg = k0; seg < k1;) {
+        const int64_t first_page = seg >> shift;
+        const int64_t seg_end = min(k1, (first_page + kPageList) << shift);
+        // the segment's pages; one that is not there is read as page 0 and its keys count as NaN
+        __syncthreads();
+        int bad = 0;
+        {
+            const int64_t e = first_page + tid;
+            if ((e << shift) < seg_end) {
+                const int p = e < a.lanes.table_width ? table[e] : -1;
+                const bool ok = uint32_t(p) < uint32_t(a.cache.pages);
+                page_list[tid] = ok ? p : -1;
+                bad = !ok;
+            }
+        }
+        const bool any_bad = __syncthreads_or(bad);
+        int at_tile = 0;   // of the list's tokens
+
+        const int64_t list_at = first_page << shift;   // the list's first token
+        const int last_token = int(seg_end - 1 - list_at);
+        auto load_tile = [&](int64_t at, int stage) {
+            const int rel = int(at - list_at);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int r0 = (wave * kLoads + j) * kRowsPerLoad, r = r0 + lane / kChunks;
+                const int token = min(rel + r, last_token);   // (past the end: the last key again, masked)
+                const int page = max(page_list[token >> shift], 0);
+                const int64_t o = int64_t(page) * a.cache.page_stride + head_offset +
+                                  int64_t(token & (ps - 1)) * a.cache.token_stride +
+                                  ((lane % kChunks) ^ swizzle<D>(r)) * 8;
+                load_to_lds(static_cast<const uint16_t*>(a.cache.keys) + o, &tiles[stage][0][r0 * D * 2]);
+                load_to_lds(static_cast<const uint16_t*>(a.cache.values) + o, &tiles[stage][1][r0 * D * 2]);
+            }
+        };
+
+        // One block or two of 32 keys: scores, weights, values.  Where rows do not see
+        // every key (kMasked, one block): `end` and `known` are the tile's keys that
+        // there are and that every row sees.
+        auto attend = [&]<int kN, bool kMasked>(int stage, int b0, int step, int end, int known) {
+            f32x16_t sc[kN];
+            // LDS addresses of the lane's first key chunk and of its first values; chunk 2 k + half
+            // and block d of 32 places are these with bits flipped.  (Kept from the optimiser,
+            // which would hold all of them in registers through the loop.)
+            uint32_t key_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + key_lane;
+            uint32_t value_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + kTileBytes + value_lane;
+            asm volatile("" : "+v"(key_at), "+v"(value_at));
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+                    sc[n] = mfma<DT>(*lds_ptr<s16x8_t>((key_at ^ (k << 5)) + (b0 + n * step) * (64 * D)), qf[k], sc[n]);
+            }
+            uint32_t visible = ~0u;   // bit 8 (i / 4) + i % 4: score i
+            if constexpr (kMasked) {
+                const int key = b0 * 32 + col;   // keys whose page is not there count as NaN
+                const bool lost = any_bad && key < end && page_list[(at_tile + key) >> shift] < 0;
+                const uint32_t gone = uint32_t(ballot(lost));
+                const int there = end - b0 * 32, before = known - b0 * 32;   // of this block
+                uint64_t w;   // the block's keys that the lane's query sees
+                if (a.tree && !is_prefix) w = before >= 32 ? ~0ull : before <= -64 ? 0ull : before < 0 ? seen >> -before : seen << before | low_bits(before);
+                else w = low_bits(before + own_row + 1) | (is_prefix ? ~0ull : 0ull);
+                w &= low_bits(there);
+                visible = uint32_t(w) >> (4 * half);
+                const uint32_t nan = gone >> (4 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float score = sc[0][i];
+                    const uint32_t x = __builtin_bit_cast(uint32_t, score) | (bit_mask(nan, 8 * (i / 4) + i % 4) >> 1);
+                    const uint32_t see = bit_mask(visible, 8 * (i / 4) + i % 4);
+                    sc[0][i] = __builtin_bit_cast(float, (x & see) | (0xff800000u & ~see));
+                }
+            }
+            float tile_top = -kInfF;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) tile_top = fmaxf(tile_top, sc[n][i]);
+            tile_top = halves_max(tile_top);
+            const bool raise = (tile_top - top) * a.scale2 > kSlack || top == -kInfF;
+            if (ballot(raise)) {
+                const float next = raise ? fmaxf(top, tile_top) : top;
+                const float shrink = rescale(top, next, a.scale2);
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+                top = next;
+            }
+            const float offset = top == -kInfF ? 0.0f : top * a.scale2;
+            s16x8_t pf[kN][2];
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], a.scale2, -offset));
+                    if constexpr (kMasked)
+                        p[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[i]) &
+                                                             bit_mask(visible, 8 * (i / 4) + i % 4));
+                    sum += p[i];
+                }
+                pf[n][0] = pack8<DT>(p);
+                pf[n][1] = pack8<DT>(p + 8);
+            }
+            // values that are no numbers must reach the rows that see them, and no others (0 x Inf is
+            // NaN): they count as 0 here, and the part is marked for the join
+            bool dirty = false;
+            if constexpr (kMasked) {
+                const uint4* const v = reinterpret_cast<const uint4*>(&tiles[stage][1][b0 * 64 * D]);
+                uint32_t any = 0;
+                for (int i = lane; i < 32 * D / 8; i += kWave) {
+                    const uint4 x = v[i];
+                    any |= uint32_t(any_nonfinite<DT>(x));
+                }
+                dirty = ballot(any != 0);
+                marked |= dirty;
+            }
+            auto value_fragment = [&](int kb, int n, int d) {
+                const uint32_t o = uint32_t((b0 + n * step) * 32 + kb * 16) * (2 * D);
+                const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((value_at ^ (d << 6)) + o));
+                const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    lds_ptr<s16x4_t>((value_at ^ (d << 6) ^ kValueFlip) + 16 * D + o));
+                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int d = 0; d < kOuts; ++d) {
+                        s16x8_t vf = value_fragment(kb, n, d);
+                        if (kMasked && dirty) vf = finite_or_zero<DT>(vf);
+                        acc[d] = mfma<DT>(vf, pf[n][kb], acc[d]);
+                    }
+                }
+            }
+        };
+
+        load_tile(seg, 0);
+        int stage = 0;
+        int64_t at = seg;
+        auto arrive = [&] {
+            loads_done();      // this wave's part of the tile has arrived
+            __syncthreads();   // everyone's has, and the other stage is no longer read
+            if (at + kKeys < seg_end) load_tile(at + kKeys, stage ^ 1);
+        };
+        // tiles that every row sees whole, then the others (two loops: each has its own registers)
+        const int64_t whole = any_bad ? seg : min(seg_end, s.context);
+        for (; at + kKeys <= whole; at += kKeys, stage ^= 1) {
+            arrive();
+            if (!active) continue;
+            if (kBlocks / along_keys >= 2) {
+                for (int b = ki; b < kBlocks; b += 2 * along_keys)
+                    attend.template operator()<2, false>(stage, b, along_keys, kKeys, kKeys);
+            } else {
+                attend.template operator()<1, false>(stage, ki, 1, kKeys, kKeys);
+            }
+        }
+        for (; at < seg_end; at += kKeys, stage ^= 1) {
+            arrive();
+            if (!active) continue;
+            at_tile = int(at - list_at);
+            const int end = int(min(seg_end - at, int64_t(kKeys)));
+            const int known = int(max(min(s.context - at, int64_t(kKeys)), int64_t(-(1 << 30))));
+            for (int b = ki; b < kBlocks; b += along_keys) attend.template operator()<1, true>(stage, b, 1, end, known);
+        }
+        seg = seg_end;
+    }
+
+    // the waves that shared queries join
+    if (along_keys > 1) {
+        __syncthreads();
+        float* const mem = reinterpret_cast<float*>(tiles);
+        constexpr int kPer = kOuts * 16 + 2;   // floats a lane leaves
+        float* const slot = mem + (wave - plan.waves) * kPer * kWave + lane;
+        if (active && ki > 0) {
+#pragma unroll
+            for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) slot[(d * 16 + i) * kWave] = acc[d][i];
+            slot[kOuts * 16 * kWave] = top;
+            slot[(kOuts * 16 + 1) * kWave] = marked ? -sum : sum;
+        }
+        __syncthreads();
+        if (!active || ki > 0) return;
+        for (int k = 1; k < along_keys; ++k) {
+            const float* const other = mem + ((k - 1) * plan.waves + qi) * kPer * kWave + lane;
+            const float ot = other[kOuts * 16 * kWave], left = other[(kOuts * 16 + 1) * kWave], os = fabsf(left);
+            marked |= __builtin_signbit(left);
+            const float next = fmaxf(top, ot);
+            const float x = rescale(top, next, a.scale2), y = rescale(ot, next, a.scale2);
+            top = next;
+            sum = sum * x + os * y;
+#pragma unroll
+            for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * x + other[(d * 16 + i) * kWave] * y;
+        }
+    }
+    if (!live || ki > 0) return;
+    sum = halves_sum(sum);
+    marked = halves_max(marked ? 1.0f : 0.0f) > 0.0f;
+    const int64_t at = int64_t(row) * a.heads + qhead;
+    const int64_t part = (is_prefix ? split : a.plan.prefix.splits + split) * (int64_t(a.lanes.rows) * a.heads) + at;
+    if (half == 0) a.part_ml[part] = make_float2(top, marked ? -sum : sum);
+    float* const o = a.part_o + part * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(o + d * 32 + 2 * i) =
+                make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+}
+
+// The infinities and NaN among the values of a marked part that the row sees, in
+// places d .. d + 3 of its head.
+template <int DT>
+__device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, const ScopePlan& plan, int split, int row,
+                                          int head, int d, bool is_prefix) {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int64_t k0, k1;
+    part_range(s, plan, split, &k0, &k1);
+    const int i = row - s.row0;
+    const uint64_t seen = a.tree && !is_prefix ? a.tree[row] : 0;
+    for (int64_t key = k0; key < k1; ++key) {
+        const int64_t j = key - s.context;
+        if (!(j < 0 || (a.tree ? j < 64 && (seen >> (j & 63) & 1) : j <= i))) continue;
+        const int page = page_of(a.lanes, a.cache.pages, a.cache.page_size, s.table, key);
+        if (page < 0) continue;
+        const uint16_t* const v = static_cast<const uint16_t*>(a.cache.values) + int64_t(page) * a.cache.page_stride +
+                                  int64_t(head / (a.heads / a.cache.kv_heads)) * a.cache.head_stride +
+                                  (key & (a.cache.page_size - 1)) * a.cache.token_stride + d;
+        for (int e = 0; e < 4; ++e)
+            if (!Elem<DT>::finite_bits(v[e])) x[e] += Elem<DT>::decode(v[e]);
+    }
+    return make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// The parts of every (row, head) joined.  D / 4 threads a pair.
+template <int DT, int D>
+__global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
+    constexpr int kPer = D / 4;
+    const int64_t at = int64_t(blockIdx.x) * (kAttnThreads / kPer) + threadIdx.x / kPer;
+    const int d = threadIdx.x % kPer * 4;
+    const int64_t pairs = int64_t(a.lanes.rows) * a.heads;
+    const int row = int(at / a.heads), head = int(at % a.heads);
+    if (at >= pairs || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
+    const int lane = lane_of_row(a.lanes.row_offsets, a.lanes.lanes, row);
+    const Scope own = own_scope(a, lane);
+    bool bad = row - own.row0 >= a.max_rows;
+    int used[2] = {0, 0};
+    Scope shared{};
+    if (a.groups) {
+        const int g = lane_of_row(a.group_offsets, a.groups, lane);
+        if (lane >= a.group_offsets[g] && lane < a.group_offsets[g + 1]) {
+            shared = prefix_scope(a, g);
+            if (shared.end > 0) {
+                bad |= row - shared.row0 >= a.max_group_rows;
+                used[0] = int(min(int64_t(a.plan.prefix.splits), (shared.end + a.plan.prefix.chunk - 1) / a.plan.prefix.chunk));
+            }
+        }
+    }
+    used[1] = int(min(int64_t(a.plan.own.splits), (own.end - own.begin + a.plan.own.chunk - 1) / a.plan.own.chunk));
+    float top = -kInfF, sum = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    if (!bad) {
+        for (int k = 0; k < 2; ++k) {
+            const int64_t first = k ? a.plan.prefix.splits : 0;
+            for (int i = 0; i < used[k]; ++i) {
+                float2 ml = a.part_ml[(first + i) * pairs + at];
+                float4 v = *reinterpret_cast<const float4*>(a.part_o + ((first + i) * pairs + at) * D + d);
+                if (__builtin_signbit(ml.y)) {
+                    ml.y = -ml.y;
+                    const float4 x = no_numbers<DT>(a, k ? own : shared, k ? a.plan.own : a.plan.prefix, i, row, head, d, !k);
+                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+                }
+                if (ml.x == -kInfF && ml.y == 0.0f) continue;   // it saw nothing
+                const float next = fmaxf(top, ml.x);
+                const float x = rescale(top, next, a.scale2), y = rescale(ml.x, next, a.scale2);
+                top = next;
+                sum = sum * x + ml.y * y;
+                o.x = o.x * x + v.x * y; o.y = o.y * x + v.y * y;
+                o.z = o.z * x + v.z * y; o.w = o.w * x + v.w * y;
+            }
+        }
+    } else {
+        sum = __builtin_nanf("");
+    }
+    const bool empty = sum == 0.0f;
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    uint16_t* const out = static_cast<uint16_t*>(a.out) + int64_t(row) * a.out_row + int64_t(head) * a.out_head + d;
+    uint2 w;
+    w.x = Elem<DT>::round(o.x * inv) | Elem<DT>::round(o.y * inv) << 16;
+    w.y = Elem<DT>::round(o.z * inv) | Elem<DT>::round(o.w * inv) << 16;
+    *reinterpret_cast<uint2*>(out) = w;
+    if (a.lse && d == 0) a.lse[at] = empty ? -kInfF : (top * a.scale2 + log2f(sum)) * (1.0f / kLog2e);
+}
+
+ScopePlan scope_plan(int64_t queries) {
+    ScopePlan p{};
+    p.waves = queries <= 32 ? 1 : queries <= 64 ? 2 : 4;
+    p.tiles = int((queries + 32 * p.waves - 1) / (32 * p.waves));
+    return p;
+}
+// How the work is cut: chunks of one length, so that about two workgroups a CU
+// have one each, but none shorter than two tiles of the keys.
+AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int groups, int max_rows, int max_group_rows,
+                        int64_t max_own, int64_t max_prefix) {
+    AttnPlan p{};
+    const int per_kv = heads / kv_heads, tile = kTileBytes / (2 * head_dim);
+    p.own = scope_plan(int64_t(max_rows) * per_kv);
+    p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv);
+    const int64_t own_items = int64_t(lanes) * kv_heads * p.own.tiles;
+    const int64_t prefix_items = int64_t(groups) * kv_heads * p.prefix.tiles;
+    const int64_t work = own_items * max_own + prefix_items * max_prefix;
+    int64_t chunk = std::max<int64_t>(work / 512, 2 * tile);
+    chunk = int64_t(align_up(size_t(chunk), size_t(tile)));
+    p.own.chunk = p.prefix.chunk = int(std::min<int64_t>(chunk, 1 << 30));
+    p.own.splits = int(std::clamp<int64_t>((max_own + chunk - 1) / chunk, 1, 128));
+    p.prefix.splits = groups ? int(std::clamp<int64_t>((max_prefix + chunk - 1) / chunk, 1, 128)) : 0;
+    return p;
+}
+
+template <int DT, int D> void launch_dim(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+    hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(kAttnThreads), 0, stream, a);
+    const int64_t pairs = int64_t(a.lanes.rows) * a.heads, per = kAttnThreads / (D / 4);
+    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((pairs + per - 1) / per)), dim3(kAttnThreads), 0, stream, a);
+}
+template <int DT> void launch_type(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
+    switch (a.cache.head_dim) {
+        case 64: launch_dim<DT, 64>(a, blocks, stream); break;
+        case 128: launch_dim<DT, 128>(a, blocks, stream); break;
+        default: launch_dim<DT, 256>(a, blocks, stream); break;
+    }
 }
 
 }  // namespace
 
 size_t attention_workspace(int rows, int heads, int kv_heads, int head_dim, int lanes, int groups, int max_rows,
                            int max_group_rows, int64_t max_own, int64_t max_prefix) {
-    return 256;
+    const AttnPlan p = attention_plan(heads, kv_heads, head_dim, lanes, groups, max_rows, max_group_rows, max_own,
+                                      max_prefix);
+    const size_t pairs = size_t(rows) * heads * p.parts();
+    return align_up(pairs * head_dim * 4, 256) + align_up(pairs * 8, 256) + 256;
 }
 
 vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, int heads, const vi_head_rows& q,
@@ -99,12 +606,25 @@ vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, 
                            int max_rows, int max_group_rows, int64_t max_own, int64_t max_prefix,
                            const uint64_t* tree, void* out, int64_t out_row, int64_t out_head, float* lse, void* ws,
                            size_t ws_bytes, hipStream_t stream) {
-    AttnArgs a{cache, lanes, q, heads, groups, scale, group_offsets, prefix_lens, max_rows, max_group_rows, tree, out,
-               out_row, out_head, lse};
-    const int64_t blocks = int64_t(lanes.rows) * heads;
-    if (blocks > 0x7fffffff) return VI_ERR_UNSUPPORTED;
-    auto* kernel = cache.dtype == VI_BF16 ? attention_row_kernel<VI_BF16> : attention_row_kernel<VI_F16>;
-    hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(64), 0, stream, a);
+    AttnArgs a{};
+    a.cache = cache; a.lanes = lanes; a.q = q; a.heads = heads; a.groups = groups;
+    a.scale2 = __builtin_fabsf(scale) * kLog2e;
+    a.flip = __builtin_signbit(scale) ? 0x80008000u : 0u;
+    a.group_offsets = group_offsets; a.prefix_lens = prefix_lens;
+    a.max_rows = max_rows; a.max_group_rows = max_group_rows; a.tree = tree;
+    a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse;
+    a.plan = attention_plan(heads, cache.kv_heads, cache.head_dim, lanes.lanes, groups, max_rows, max_group_rows, max_own,
+                            max_prefix);
+    const size_t pairs = size_t(lanes.rows) * heads * a.plan.parts();
+    Carver c(ws, ws_bytes);
+    a.part_o = c.take<float>(pairs * cache.head_dim);
+    a.part_ml = c.take<float2>(pairs);
+    if (!c.ok) return VI_ERR_WORKSPACE;
+    const int64_t blocks = (int64_t(groups) * a.plan.prefix.tiles * a.plan.prefix.splits +
+                            int64_t(lanes.lanes) * a.plan.own.tiles * a.plan.own.splits) * cache.kv_heads;
+    if (blocks > 0x7fffffff || pairs > 0x7fffffffffull) return VI_ERR_UNSUPPORTED;
+    if (cache.dtype == VI_BF16) launch_type<VI_BF16>(a, unsigned(blocks), stream);
+    else launch_type<VI_F16>(a, unsigned(blocks), stream);
     return launch_status();
 }
 
