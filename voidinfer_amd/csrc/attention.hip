@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / kWave;
-constexpr int kPageList = 256;     // pages of a segment of the keys
 constexpr int kTileBytes = 16384;  // a tile's keys (and its values) in LDS
 constexpr float kLog2e = 1.44269504088896340736f;
 // A running maximum is raised (and the sums rescaled) only once a score exceeds
@@ -87,15 +86,16 @@ template <int DT> __device__ __forceinline__ s16x8_t pack8(const float* p) {
     }
 }
 
-// 16 bytes a lane from its address to LDS (`to`: wave-uniform, lane i's bytes at
-// 16 i), without registers in between.  In assembly because the compiler waits for
-// every such load before any later read of LDS, also of another buffer: the
-// loads of the next tile would not run beside the work on this one.  loads_done()
-// waits for the wave's own, a barrier behind it for everyone's.
-__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+// 16 bytes a lane from base + offset to LDS (base and `to` wave-uniform, lane i's
+// bytes at to + 16 i), without registers in between.  In assembly because the
+// compiler waits for every such load before any later read of LDS, also of another
+// buffer: the loads of the next tile would not run beside the work on this one.
+// loads_done() waits for the wave's own, a barrier behind it for everyone's.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, void* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(
         uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to)));
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(at)
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -172,51 +172,47 @@ __device__ __forceinline__ Scope prefix_scope(const AttnArgs& a, int g) {
     s.end = s.context = max(a.prefix_lens[g], 0);
     return s;
 }
-// Part `split` of a scope's keys: the last takes what is left.
+// Part `split` of a scope's keys: chunks from the 16-token boundary at or below
+// the first key on (no page begins inside 16 tokens); the last takes what is left.
 __device__ __forceinline__ void part_range(const Scope& s, const ScopePlan& p, int split, int64_t* k0, int64_t* k1) {
-    *k0 = min(s.begin + int64_t(split) * p.chunk, s.end);
-    *k1 = split == p.splits - 1 ? s.end : min(*k0 + p.chunk, s.end);
+    const int64_t base = s.begin & ~int64_t(15);
+    *k0 = min(max(s.begin, base + int64_t(split) * p.chunk), s.end);
+    *k1 = split == p.splits - 1 ? s.end : max(min(base + int64_t(split + 1) * p.chunk, s.end), *k0);
+}
+__device__ __forceinline__ int parts_used(const Scope& s, const ScopePlan& p) {
+    const int64_t base = s.begin & ~int64_t(15);
+    return int(min(int64_t(p.splits), (s.end - base + p.chunk - 1) / p.chunk));
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
-    constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
-    constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
-    constexpr int kLoads = kKeys / kRowsPerLoad / kAttnWaves;           // loads of a wave for a tile's keys
-    constexpr int kSteps = D / 16, kOuts = D / 32;
-    __shared__ __align__(1024) unsigned char tiles[2][2][kTileBytes];   // [stage][keys, values]
-    __shared__ int page_list[kPageList];
+template <int D> struct Tile {
+    static constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
+    static constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
+    static constexpr int kLoads = kKeys / kRowsPerLoad / kAttnWaves;           // loads of a wave for a tile's keys
+    static constexpr int kSteps = D / 16, kOuts = D / 32;
+};
+template <int D> using Tiles = unsigned char[2][2][kTileBytes];   // [stage][keys, values]
+
+// One item: queries m0 .. of the scope's over keys k0 .. k1.  kWaves of the workgroup's
+// waves hold 32 queries each; the others share the tile's blocks of keys with them.
+template <int DT, int D, int kWaves>
+__device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, const Scope& s, bool is_prefix,
+                                            int head, int queries, int m0, int64_t k0, int64_t k1, int64_t part) {
+    using T = Tile<D>;
+    constexpr int kKeys = T::kKeys, kBlocks = T::kBlocks, kChunks = T::kChunks, kRowsPerLoad = T::kRowsPerLoad;
+    constexpr int kLoads = T::kLoads, kSteps = T::kSteps, kOuts = T::kOuts;
+    constexpr int kAlong = kAttnWaves / kWaves < kBlocks ? kAttnWaves / kWaves : kBlocks;   // waves along the keys
+    constexpr int kMine = kBlocks / kAlong, kStep = kMine >= 2 ? 2 : 1;                      // a wave's blocks; at once
 
     const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int col = lane & 31, half = lane >> 5;
-    const int kv_heads = a.cache.kv_heads, per_kv = a.heads / kv_heads, ps = a.cache.page_size;
-    const int shift = __builtin_ctz(unsigned(ps));
-
-    // which item: heads fastest, so that one head's tiles stay on one XCD's L2 where heads are a multiple of 8
-    const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
-    int item = blockIdx.x;
-    const bool is_prefix = item < prefix_items;
-    if (!is_prefix) item -= prefix_items;
-    const ScopePlan& plan = is_prefix ? a.plan.prefix : a.plan.own;
-    const int head = item % kv_heads;
-    item /= kv_heads;
-    const int tile = item % plan.tiles;
-    item /= plan.tiles;
-    const int split = item % plan.splits, which = item / plan.splits;
-    const Scope s = is_prefix ? prefix_scope(a, which) : own_scope(a, which);
-    const int queries = min(s.rows, is_prefix ? a.max_group_rows : a.max_rows) * per_kv;
-    const int m0 = tile * 32 * plan.waves;
-    int64_t k0, k1;
-    part_range(s, plan, split, &k0, &k1);
-    if (m0 >= queries || k0 >= k1) return;
+    const int per_kv = a.heads / a.cache.kv_heads, ps = a.cache.page_size, shift = __builtin_ctz(unsigned(ps));
 
     // the wave's queries and its blocks of a tile's keys
-    const int along_keys = min(kAttnWaves / plan.waves, kBlocks);
-    const int qi = wave % plan.waves, ki = wave / plan.waves;
+    const int qi = wave % kWaves, ki = wave / kWaves;
     const int m = m0 + qi * 32 + col;
-    const bool active = m0 + qi * 32 < queries && ki < along_keys;
+    const bool active = m0 + qi * 32 < queries && ki < kAlong;
     const bool live = active && m < queries;
-    const int row = s.row0 + (live ? m / per_kv : 0), own_row = live ? m / per_kv : 0;
+    const int own_row = live ? m / per_kv : 0, row = s.row0 + own_row;
     const int qhead = head * per_kv + (live ? m % per_kv : 0);
     s16x8_t qf[kSteps];
     {
@@ -249,199 +245,201 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(
     float top = -kInfF, sum = 0.0f;   // raw score units; this half's sum
     bool marked = false;
 
+    // Tiles begin at multiples of 16 tokens, so the rows of one load lie in one page:
+    // its address is uniform, the lane's part of it fixed.  Lane j of a wave looks up
+    // the page of load j, a tile ahead of the load.
+    const int64_t origin = k0 & ~int64_t(15);
+    const int total = int((k1 - origin + kKeys - 1) / kKeys);
+    const int64_t all_see = min(k1, s.context);
+    const int first = origin < k0 ? 1 : 0;                                   // the whole tiles: every row sees every key
+    const int whole = max(int((all_see - origin) / kKeys), first) - first;   // these come first,
+    auto tile_of = [&](int i) { return first + i < total ? first + i : 0; };  // then those behind, then the first
     const int32_t* const table = a.lanes.tables + int64_t(s.table) * a.lanes.table_stride;
-    const int64_t head_offset = int64_t(head) * a.cache.head_stride;
-
-    for (int64_t seg = k0; seg < k1;) {
-        const int64_t first_page = seg >> shift;
-        const int64_t seg_end = min(k1, (first_page + kPageList) << shift);
-        // the segment's pages; one that is not there is read as page 0 and its keys count as NaN
-        __syncthreads();
-        int bad = 0;
-        {
-            const int64_t e = first_page + tid;
-            if ((e << shift) < seg_end) {
-                const int p = e < a.lanes.table_width ? table[e] : -1;
-                const bool ok = uint32_t(p) < uint32_t(a.cache.pages);
-                page_list[tid] = ok ? p : -1;
-                bad = !ok;
-            }
-        }
-        const bool any_bad = __syncthreads_or(bad);
-        int at_tile = 0;   // of the list's tokens
-
-        const int64_t list_at = first_page << shift;   // the list's first token
-        const int last_token = int(seg_end - 1 - list_at);
-        auto load_tile = [&](int64_t at, int stage) {
-            const int rel = int(at - list_at);
+    const unsigned char* const keys_at = static_cast<const unsigned char*>(a.cache.keys) + 2 * int64_t(head) * a.cache.head_stride;
+    const unsigned char* const values_at = static_cast<const unsigned char*>(a.cache.values) + 2 * int64_t(head) * a.cache.head_stride;
+    uint32_t from_lane[kLoads];
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const int r0 = (wave * kLoads + j) * kRowsPerLoad, r = r0 + lane / kChunks;
-                const int token = min(rel + r, last_token);   // (past the end: the last key again, masked)
-                const int page = max(page_list[token >> shift], 0);
-                const int64_t o = int64_t(page) * a.cache.page_stride + head_offset +
-                                  int64_t(token & (ps - 1)) * a.cache.token_stride +
-                                  ((lane % kChunks) ^ swizzle<D>(r)) * 8;
-                load_to_lds(static_cast<const uint16_t*>(a.cache.keys) + o, &tiles[stage][0][r0 * D * 2]);
-                load_to_lds(static_cast<const uint16_t*>(a.cache.values) + o, &tiles[stage][1][r0 * D * 2]);
-            }
-        };
-
-        // One block or two of 32 keys: scores, weights, values.  Where rows do not see
-        // every key (kMasked, one block): `end` and `known` are the tile's keys that
-        // there are and that every row sees.
-        auto attend = [&]<int kN, bool kMasked>(int stage, int b0, int step, int end, int known) {
-            f32x16_t sc[kN];
-            // LDS addresses of the lane's first key chunk and of its first values; chunk 2 k + half
-            // and block d of 32 places are these with bits flipped.  (Kept from the optimiser,
-            // which would hold all of them in registers through the loop.)
-            uint32_t key_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + key_lane;
-            uint32_t value_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + kTileBytes + value_lane;
-            asm volatile("" : "+v"(key_at), "+v"(value_at));
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-                    sc[n] = mfma<DT>(*lds_ptr<s16x8_t>((key_at ^ (k << 5)) + (b0 + n * step) * (64 * D)), qf[k], sc[n]);
-            }
-            uint32_t visible = ~0u;   // bit 8 (i / 4) + i % 4: score i
-            if constexpr (kMasked) {
-                const int key = b0 * 32 + col;   // keys whose page is not there count as NaN
-                const bool lost = any_bad && key < end && page_list[(at_tile + key) >> shift] < 0;
-                const uint32_t gone = uint32_t(ballot(lost));
-                const int there = end - b0 * 32, before = known - b0 * 32;   // of this block
-                uint64_t w;   // the block's keys that the lane's query sees
-                if (a.tree && !is_prefix) w = before >= 32 ? ~0ull : before <= -64 ? 0ull : before < 0 ? seen >> -before : seen << before | low_bits(before);
-                else w = low_bits(before + own_row + 1) | (is_prefix ? ~0ull : 0ull);
-                w &= low_bits(there);
-                visible = uint32_t(w) >> (4 * half);
-                const uint32_t nan = gone >> (4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float score = sc[0][i];
-                    const uint32_t x = __builtin_bit_cast(uint32_t, score) | (bit_mask(nan, 8 * (i / 4) + i % 4) >> 1);
-                    const uint32_t see = bit_mask(visible, 8 * (i / 4) + i % 4);
-                    sc[0][i] = __builtin_bit_cast(float, (x & see) | (0xff800000u & ~see));
-                }
-            }
-            float tile_top = -kInfF;
-#pragma unroll
-            for (int n = 0; n < kN; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) tile_top = fmaxf(tile_top, sc[n][i]);
-            tile_top = halves_max(tile_top);
-            const bool raise = (tile_top - top) * a.scale2 > kSlack || top == -kInfF;
-            if (ballot(raise)) {
-                const float next = raise ? fmaxf(top, tile_top) : top;
-                const float shrink = rescale(top, next, a.scale2);
-                sum *= shrink;
-#pragma unroll
-                for (int d = 0; d < kOuts; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
-                top = next;
-            }
-            const float offset = top == -kInfF ? 0.0f : top * a.scale2;
-            s16x8_t pf[kN][2];
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-                float p[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], a.scale2, -offset));
-                    if constexpr (kMasked)
-                        p[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[i]) &
-                                                             bit_mask(visible, 8 * (i / 4) + i % 4));
-                    sum += p[i];
-                }
-                pf[n][0] = pack8<DT>(p);
-                pf[n][1] = pack8<DT>(p + 8);
-            }
-            // values that are no numbers must reach the rows that see them, and no others (0 x Inf is
-            // NaN): they count as 0 here, and the part is marked for the join
-            bool dirty = false;
-            if constexpr (kMasked) {
-                const uint4* const v = reinterpret_cast<const uint4*>(&tiles[stage][1][b0 * 64 * D]);
-                uint32_t any = 0;
-                for (int i = lane; i < 32 * D / 8; i += kWave) {
-                    const uint4 x = v[i];
-                    any |= uint32_t(any_nonfinite<DT>(x));
-                }
-                dirty = ballot(any != 0);
-                marked |= dirty;
-            }
-            auto value_fragment = [&](int kb, int n, int d) {
-                const uint32_t o = uint32_t((b0 + n * step) * 32 + kb * 16) * (2 * D);
-                const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((value_at ^ (d << 6)) + o));
-                const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    lds_ptr<s16x4_t>((value_at ^ (d << 6) ^ kValueFlip) + 16 * D + o));
-                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            };
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int d = 0; d < kOuts; ++d) {
-                        s16x8_t vf = value_fragment(kb, n, d);
-                        if (kMasked && dirty) vf = finite_or_zero<DT>(vf);
-                        acc[d] = mfma<DT>(vf, pf[n][kb], acc[d]);
-                    }
-                }
-            }
-        };
-
-        load_tile(seg, 0);
-        int stage = 0;
-        int64_t at = seg;
-        auto arrive = [&] {
-            loads_done();      // this wave's part of the tile has arrived
-            __syncthreads();   // everyone's has, and the other stage is no longer read
-            if (at + kKeys < seg_end) load_tile(at + kKeys, stage ^ 1);
-        };
-        // tiles that every row sees whole, then the others (two loops: each has its own registers)
-        const int64_t whole = any_bad ? seg : min(seg_end, s.context);
-        for (; at + kKeys <= whole; at += kKeys, stage ^= 1) {
-            arrive();
-            if (!active) continue;
-            if (kBlocks / along_keys >= 2) {
-                for (int b = ki; b < kBlocks; b += 2 * along_keys)
-                    attend.template operator()<2, false>(stage, b, along_keys, kKeys, kKeys);
-            } else {
-                attend.template operator()<1, false>(stage, ki, 1, kKeys, kKeys);
-            }
-        }
-        for (; at < seg_end; at += kKeys, stage ^= 1) {
-            arrive();
-            if (!active) continue;
-            at_tile = int(at - list_at);
-            const int end = int(min(seg_end - at, int64_t(kKeys)));
-            const int known = int(max(min(s.context - at, int64_t(kKeys)), int64_t(-(1 << 30))));
-            for (int b = ki; b < kBlocks; b += along_keys) attend.template operator()<1, true>(stage, b, 1, end, known);
-        }
-        seg = seg_end;
+    for (int j = 0; j < kLoads; ++j) {
+        const int r = lane / kChunks;
+        from_lane[j] = uint32_t(2 * r * a.cache.token_stride) +
+                       (uint32_t((lane % kChunks) ^ swizzle<D>((wave * kLoads + j) * kRowsPerLoad + r)) << 4);
     }
+    auto look_up = [&](int i) {   // (past the end: the last key's page, masked)
+        const int64_t key = origin + int64_t(tile_of(min(i, total - 1))) * kKeys + (wave * kLoads + (lane & (kLoads - 1))) * kRowsPerLoad;
+        const int64_t e = min(key, k1 - 1) >> shift;
+        return e < a.lanes.table_width ? table[e] : -1;
+    };
+    auto load_tile = [&](int i, int stage, int pages) {
+        const int first_place = int(origin + int64_t(tile_of(i)) * kKeys) & (ps - 1);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int r0 = (wave * kLoads + j) * kRowsPerLoad;
+            const int page = __builtin_amdgcn_readlane(pages, j);
+            unsigned char* const kt = &tiles[stage][0][r0 * D * 2];
+            unsigned char* const vt = &tiles[stage][1][r0 * D * 2];
+            if (uint32_t(page) < uint32_t(a.cache.pages)) {
+                const int64_t o = 2 * (int64_t(page) * a.cache.page_stride +
+                                       int64_t((first_place + r0) & (ps - 1)) * a.cache.token_stride);
+                load_to_lds(keys_at + o, from_lane[j], kt);
+                load_to_lds(values_at + o, from_lane[j], vt);
+            } else {   // no such page: keys that are NaN, so that rows that see them are
+                reinterpret_cast<uint4*>(kt)[lane] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                reinterpret_cast<uint4*>(vt)[lane] = make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
 
-    // the waves that shared queries join
-    if (along_keys > 1) {
-        __syncthreads();
-        float* const mem = reinterpret_cast<float*>(tiles);
-        constexpr int kPer = kOuts * 16 + 2;   // floats a lane leaves
-        float* const slot = mem + (wave - plan.waves) * kPer * kWave + lane;
-        if (active && ki > 0) {
+    // One block or two of 32 keys: scores, weights, values.  Where rows do not see
+    // every key (kMasked): of the tile's keys there are those from `begin` on and below
+    // `end`, and every row sees those below `known`.
+    auto attend = [&]<int kN, bool kMasked>(int stage, int b0, int begin, int end, int known) {
+        // LDS addresses of the lane's first key chunk and of its first values; chunk 2 k + half
+        // and block d of 32 places are these with bits flipped.  (Kept from the optimiser,
+        // which would hold all of them in registers through the loop.)
+        uint32_t key_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + key_lane;
+        uint32_t value_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + kTileBytes + value_lane;
+        asm volatile("" : "+v"(key_at), "+v"(value_at));
+        f32x16_t sc[kN];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            s16x8_t kf[kSteps];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) kf[k] = *lds_ptr<s16x8_t>((key_at ^ (k << 5)) + (b0 + n * kAlong) * (64 * D));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) sc[n] = mfma<DT>(kf[k], qf[k], sc[n]);
+        }
+        uint32_t visible = ~0u;   // bit 8 (i / 4) + i % 4: score i
+        if constexpr (kMasked) {
+            static_assert(kN == 1);
+            const int before = known - b0 * 32;   // of this block
+            uint64_t w;   // the block's keys that the lane's query sees
+            if (is_prefix) w = ~0ull;
+            else if (!a.tree) w = low_bits(before + own_row + 1);
+            else if (before >= 0) w = before >= 32 ? ~0ull : seen << before | low_bits(before);
+            else w = before > -64 ? seen >> -before : 0ull;
+            w &= low_bits(end - b0 * 32) & ~low_bits(begin - b0 * 32);
+            visible = uint32_t(w) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float score = sc[0][i];
+                const uint32_t see = bit_mask(visible, 8 * (i / 4) + i % 4);
+                sc[0][i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & see) | (0xff800000u & ~see));
+            }
+        }
+        float tile_top = -kInfF;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tile_top = fmaxf(tile_top, sc[n][i]);
+        tile_top = halves_max(tile_top);
+        const bool raise = (tile_top - top) * a.scale2 > kSlack || top == -kInfF;
+        if (ballot(raise)) {
+            const float next = raise ? fmaxf(top, tile_top) : top;
+            const float shrink = rescale(top, next, a.scale2);
+            sum *= shrink;
 #pragma unroll
             for (int d = 0; d < kOuts; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) slot[(d * 16 + i) * kWave] = acc[d][i];
+                for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
+            top = next;
+        }
+        const float offset = top == -kInfF ? 0.0f : top * a.scale2;
+        s16x8_t pf[kN][2];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], a.scale2, -offset));
+                if constexpr (kMasked)
+                    p[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[i]) &
+                                                         bit_mask(visible, 8 * (i / 4) + i % 4));
+                sum += p[i];
+            }
+            pf[n][0] = pack8<DT>(p);
+            pf[n][1] = pack8<DT>(p + 8);
+        }
+        // values that are no numbers must reach the rows that see them, and no others (0 x Inf is
+        // NaN): they count as 0 here, and the part is marked for the join
+        bool dirty = false;
+        if constexpr (kMasked) {
+            const uint4* const v = reinterpret_cast<const uint4*>(&tiles[stage][1][b0 * 64 * D]);
+            bool any = false, there = false;
+            for (int i = lane; i < 32 * kChunks; i += kWave) {
+                const bool no_number = any_nonfinite<DT>(v[i]);
+                const int key = b0 * 32 + i / kChunks;
+                any |= no_number;
+                there |= no_number && key >= begin && key < end;
+            }
+            dirty = ballot(any);
+            marked |= ballot(there) != 0;
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const uint32_t o = uint32_t((b0 + n * kAlong) * 32 + kb * 16) * (2 * D);
+                s16x8_t vf[kOuts];
+#pragma unroll
+                for (int d = 0; d < kOuts; ++d) {
+                    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((value_at ^ (d << 6)) + o));
+                    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        lds_ptr<s16x4_t>((value_at ^ (d << 6) ^ kValueFlip) + 16 * D + o));
+                    vf[d] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if (kMasked && dirty) vf[d] = finite_or_zero<DT>(vf[d]);
+                }
+#pragma unroll
+                for (int d = 0; d < kOuts; ++d) acc[d] = mfma<DT>(vf[d], pf[n][kb], acc[d]);
+            }
+        }
+    };
+
+    int pages = look_up(0), stage = 0, i = 0;
+    load_tile(0, 0, pages);
+    pages = look_up(1);
+    auto arrive = [&] {
+        loads_done();      // this wave's part of the tile has arrived
+        __syncthreads();   // everyone's has, and the other stage is no longer read
+        if (i + 1 < total) load_tile(i + 1, stage ^ 1, pages);
+        pages = look_up(i + 2);
+    };
+    // (two loops: each has its own registers)
+    for (; i < whole; ++i, stage ^= 1) {
+        arrive();
+        if (!active) continue;
+#pragma unroll
+        for (int b = 0; b < kMine; b += kStep) attend.template operator()<kStep, false>(stage, ki + b * kAlong, 0, 0, 0);
+    }
+    for (; i < total; ++i, stage ^= 1) {
+        arrive();
+        if (!active) continue;
+        const int64_t at = origin + int64_t(tile_of(i)) * kKeys;
+        const int begin = int(max(k0 - at, int64_t(0))), end = int(min(k1 - at, int64_t(kKeys)));
+        const int known = int(max(min(s.context - at, int64_t(kKeys)), int64_t(-(1 << 30))));
+        for (int b = 0; b < kMine; ++b) attend.template operator()<1, true>(stage, ki + b * kAlong, begin, end, known);
+    }
+
+    // the waves that shared queries join
+    if constexpr (kAlong > 1) {
+        __syncthreads();
+        float* const mem = reinterpret_cast<float*>(tiles);
+        constexpr int kPer = kOuts * 16 + 2;   // floats a lane leaves
+        if (active && ki > 0) {
+            float* const slot = mem + (wave - kWaves) * kPer * kWave + lane;
+#pragma unroll
+            for (int d = 0; d < kOuts; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) slot[(d * 16 + e) * kWave] = acc[d][e];
             slot[kOuts * 16 * kWave] = top;
             slot[(kOuts * 16 + 1) * kWave] = marked ? -sum : sum;
         }
         __syncthreads();
         if (!active || ki > 0) return;
-        for (int k = 1; k < along_keys; ++k) {
-            const float* const other = mem + ((k - 1) * plan.waves + qi) * kPer * kWave + lane;
+#pragma unroll
+        for (int k = 1; k < kAlong; ++k) {
+            const float* const other = mem + ((k - 1) * kWaves + qi) * kPer * kWave + lane;
             const float ot = other[kOuts * 16 * kWave], left = other[(kOuts * 16 + 1) * kWave], os = fabsf(left);
             marked |= __builtin_signbit(left);
             const float next = fmaxf(top, ot);
@@ -451,22 +449,48 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(
 #pragma unroll
             for (int d = 0; d < kOuts; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * x + other[(d * 16 + i) * kWave] * y;
+                for (int e = 0; e < 16; ++e) acc[d][e] = acc[d][e] * x + other[(d * 16 + e) * kWave] * y;
         }
     }
     if (!live || ki > 0) return;
     sum = halves_sum(sum);
     marked = halves_max(marked ? 1.0f : 0.0f) > 0.0f;
-    const int64_t at = int64_t(row) * a.heads + qhead;
-    const int64_t part = (is_prefix ? split : a.plan.prefix.splits + split) * (int64_t(a.lanes.rows) * a.heads) + at;
-    if (half == 0) a.part_ml[part] = make_float2(top, marked ? -sum : sum);
-    float* const o = a.part_o + part * D + 4 * half;
+    const int64_t at = part * (int64_t(a.lanes.rows) * a.heads) + int64_t(row) * a.heads + qhead;
+    if (half == 0) a.part_ml[at] = make_float2(top, marked ? -sum : sum);
+    float* const o = a.part_o + at * D + 4 * half;
 #pragma unroll
     for (int d = 0; d < kOuts; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(o + d * 32 + 2 * i) =
-                make_float4(acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]);
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(o + d * 32 + 2 * e) =
+                make_float4(acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
+    __shared__ __align__(1024) Tiles<D> tiles;
+    // which item: heads fastest, so that one head's tiles stay on one XCD's L2 where heads are a multiple of 8
+    const int kv_heads = a.cache.kv_heads;
+    const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
+    int item = blockIdx.x;
+    const bool is_prefix = item < prefix_items;
+    if (!is_prefix) item -= prefix_items;
+    const ScopePlan& plan = is_prefix ? a.plan.prefix : a.plan.own;
+    const int head = item % kv_heads;
+    item /= kv_heads;
+    const int tile = item % plan.tiles;
+    item /= plan.tiles;
+    const int split = item % plan.splits, which = item / plan.splits;
+    const Scope s = is_prefix ? prefix_scope(a, which) : own_scope(a, which);
+    const int queries = min(s.rows, is_prefix ? a.max_group_rows : a.max_rows) * (a.heads / kv_heads);
+    const int m0 = tile * 32 * plan.waves;
+    int64_t k0, k1;
+    part_range(s, plan, split, &k0, &k1);
+    if (m0 >= queries || k0 >= k1) return;
+    const int64_t part = is_prefix ? split : a.plan.prefix.splits + split;
+    if (plan.waves == 4) attend_part<DT, D, 4>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
+    else if (plan.waves == 2) attend_part<DT, D, 2>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
+    else attend_part<DT, D, 1>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
 }
 
 // The infinities and NaN among the values of a marked part that the row sees, in
@@ -513,11 +537,11 @@ __global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
             shared = prefix_scope(a, g);
             if (shared.end > 0) {
                 bad |= row - shared.row0 >= a.max_group_rows;
-                used[0] = int(min(int64_t(a.plan.prefix.splits), (shared.end + a.plan.prefix.chunk - 1) / a.plan.prefix.chunk));
+                used[0] = parts_used(shared, a.plan.prefix);
             }
         }
     }
-    used[1] = int(min(int64_t(a.plan.own.splits), (own.end - own.begin + a.plan.own.chunk - 1) / a.plan.own.chunk));
+    used[1] = parts_used(own, a.plan.own);
     float top = -kInfF, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
     if (!bad) {
