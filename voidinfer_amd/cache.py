@@ -26,35 +26,45 @@ import torch
 
 from . import _abi
 from ._abi import check
-from .ops import _DTYPES, _int_list, _lib, _stream, workspace
+from .ops import _int_list, _lib, _stream, workspace
 
 
-def _cache_args(k_pages: torch.Tensor, v_pages: torch.Tensor) -> bytes:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or \
-            k_pages.dtype != v_pages.dtype:
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_TYPES = {torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
+
+
+def _cache_args(k_pages: torch.Tensor, v_pages: torch.Tensor, shape: torch.Size) -> bytes:
+    strides, dtype = k_pages.stride(), k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or strides != v_pages.stride() or dtype is not v_pages.dtype:
         raise ValueError("pages must be [pages, kv_heads, page_size, head_dim], keys and values alike")
-    if k_pages.stride(3) != 1 or k_pages.dtype not in _DTYPES or not k_pages.is_cuda or not v_pages.is_cuda:
+    if strides[3] != 1 or dtype not in _TYPES or not k_pages.is_cuda or not v_pages.is_cuda:
         raise ValueError("pages must be bf16 or fp16 device memory with contiguous head_dim")
-    pages, kv_heads, page_size, dim = k_pages.shape
-    sp, sh, st, _ = k_pages.stride()
-    return _abi.KV_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), sp, sh, st, _DTYPES[k_pages.dtype], pages,
-                              page_size, kv_heads, dim, 0)
+    return _abi.KV_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2],
+                              _TYPES[dtype], shape[0], shape[2], shape[1], shape[3], 0)
 
 
 def _lane_args(tables: torch.Tensor, row_offsets: torch.Tensor, context: torch.Tensor, rows: int) -> bytes:
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1 or not tables.is_cuda:
-        raise ValueError("tables must be int32 [lanes, pages per lane] with contiguous rows")
+    address, stride, lanes, width = _table_args(tables)
+    return _abi.LANE_ROWS.pack(_int_list(row_offsets, _I32, "row_offsets", lanes + 1),
+                               _int_list(context, _I32, "context", lanes), address, stride, width, lanes, rows, 0)
+
+
+def _table_args(tables: torch.Tensor) -> tuple[int, int, int, int]:
+    """(address, stride, lanes, width)"""
+    if tables.dtype is not _I32 or tables.dim() != 2 or not tables.is_cuda:
+        raise ValueError("tables must be int32 [lanes, pages per lane] device memory")
     lanes, width = tables.shape
-    return _abi.LANE_ROWS.pack(_int_list(row_offsets, torch.int32, "row_offsets", lanes + 1),
-                               _int_list(context, torch.int32, "context", lanes), tables.data_ptr(),
-                               max(tables.stride(0), width), width, lanes, rows, 0)
+    stride, one = tables.stride()
+    if one != 1 and width > 1:
+        raise ValueError("tables must have contiguous rows")
+    return tables.data_ptr(), stride if stride > width else width, lanes, width
 
 
-def _head_args(x: torch.Tensor, like: torch.Tensor, rows: int, heads: int, name: str) -> tuple[int, int, int]:
-    if x.dim() != 3 or x.dtype != like.dtype or not x.is_cuda or x.stride(2) != 1 or \
-            x.shape != (rows, heads, like.shape[3]):
+def _head_args(x: torch.Tensor, shape: tuple[int, int, int], dtype: torch.dtype, name: str) -> tuple[int, int, int]:
+    row, head, one = x.stride() if x.dim() == 3 else (0, 0, 0)
+    if one != 1 or x.dtype is not dtype or x.shape != shape or not x.is_cuda:
         raise ValueError(f"{name} must be [rows, heads, head_dim] of the pages' type, head_dim contiguous")
-    return x.data_ptr(), x.stride(0), x.stride(1)
+    return x.data_ptr(), row, head
 
 
 def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
@@ -71,35 +81,32 @@ def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     [angle rows, rotary / 2] or None (no rotation), row positions[r] (int32
     [rows]; default: the row's cache index).  A weight of None: no norm.  flags:
     int32 [rows], VI_FLAG_ERROR on rows that could not be placed."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    cache = _cache_args(k_pages, v_pages, shape)
+    kv_heads, dim = shape[1], shape[3]
     rows, heads = q.shape[0], q.shape[1]
-    cache = _cache_args(k_pages, v_pages)
-    kv_heads, dim = k_pages.shape[1], k_pages.shape[3]
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
-    rotary = angle_rows = 0
+    rotary = angle_rows = ca = sa = 0
     if cosines is not None:
-        if sines is None or cosines.shape != sines.shape or cosines.dim() != 2 or not cosines.is_contiguous() or \
-                not sines.is_contiguous() or cosines.dtype != torch.float32 or sines.dtype != torch.float32 or \
+        if sines is None or cosines.dtype is not _F32 or sines.dtype is not _F32 or cosines.dim() != 2 or \
+                cosines.shape != sines.shape or not cosines.is_contiguous() or not sines.is_contiguous() or \
                 not cosines.is_cuda or not sines.is_cuda:
             raise ValueError("cosines and sines must be contiguous fp32 [angle rows, rotary / 2] device tensors")
-        angle_rows, rotary = cosines.shape[0], 2 * cosines.shape[1]
+        angle_rows, rotary = cosines.shape
+        rotary, ca, sa = 2 * rotary, cosines.data_ptr(), sines.data_ptr()
     elif sines is not None:
         raise ValueError("sines need cosines")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != q.dtype or w.shape != (dim,) or not w.is_contiguous() or not w.is_cuda):
-            raise ValueError("norm weights must be contiguous [head_dim] of the queries' type")
-    qa = _head_args(q, k_pages, rows, heads, "q")
-    oa = _head_args(out, k_pages, rows, heads, "out")
+    qa, oa = _head_args(q, (rows, heads, dim), dtype, "q"), _head_args(out, (rows, heads, dim), dtype, "out")
     check(_lib().vi_norm_rotate_append(
         cache, _lane_args(tables, row_offsets, context, rows), heads, _abi.HEAD_ROWS.pack(*qa),
-        _abi.HEAD_ROWS.pack(*_head_args(k, k_pages, rows, kv_heads, "k")),
-        _abi.HEAD_ROWS.pack(*_head_args(v, k_pages, rows, kv_heads, "v")),
-        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-        _abi.ROTATION.pack(0 if cosines is None else cosines.data_ptr(), 0 if sines is None else sines.data_ptr(),
-                           0 if positions is None else _int_list(positions, torch.int32, "positions", rows),
-                           angle_rows, rotary, int(interleaved), 0),
-        *oa, None if flags is None else _int_list(flags, torch.int32, "flags", rows), _stream()),
-        "vi_norm_rotate_append")
+        _abi.HEAD_ROWS.pack(*_head_args(k, (rows, kv_heads, dim), dtype, "k")),
+        _abi.HEAD_ROWS.pack(*_head_args(v, (rows, kv_heads, dim), dtype, "v")),
+        None if q_weight is None else _int_list(q_weight, dtype, "q_weight", dim),
+        None if k_weight is None else _int_list(k_weight, dtype, "k_weight", dim), eps,
+        _abi.ROTATION.pack(ca, sa, 0 if positions is None else _int_list(positions, _I32, "positions", rows),
+                           angle_rows, rotary, interleaved, 0),
+        *oa, None if flags is None else _int_list(flags, _I32, "flags", rows), _stream()), "vi_norm_rotate_append")
     return out
 
 
@@ -119,58 +126,55 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     max_own: bounds of a lane's rows, and of its tokens past the shared prefix;
     max_group_rows / max_prefix: the same of a group.  scale: 1 / sqrt(d) unless
     given.  lse: fp32 [rows, heads], written when given."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    cache = _cache_args(k_pages, v_pages, shape)
+    kv_heads, dim = shape[1], shape[3]
     rows, heads = q.shape[0], q.shape[1]
-    cache = _cache_args(k_pages, v_pages)
-    kv_heads, dim = k_pages.shape[1], k_pages.shape[3]
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
-    lanes = tables.shape[0]
     groups = go = pl = 0
     if group_offsets is not None:
         if prefix_lens is None:
             raise ValueError("group_offsets need prefix_lens")
         groups = prefix_lens.numel()
-        go = _int_list(group_offsets, torch.int32, "group_offsets", groups + 1)
-        pl = _int_list(prefix_lens, torch.int32, "prefix_lens")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (rows, heads) or not lse.is_contiguous() or
+        go, pl = _int_list(group_offsets, _I32, "group_offsets", groups + 1), _int_list(prefix_lens, _I32, "prefix_lens")
+    if lse is not None and (lse.dtype is not _F32 or lse.shape != (rows, heads) or not lse.is_contiguous() or
                             not lse.is_cuda):
         raise ValueError("lse must be contiguous fp32 [rows, heads]")
-    qa = _head_args(q, k_pages, rows, heads, "q")
-    oa = _head_args(out, k_pages, rows, heads, "out")
+    qa, oa = _head_args(q, (rows, heads, dim), dtype, "q"), _head_args(out, (rows, heads, dim), dtype, "out")
+    lanes = _lane_args(tables, row_offsets, context, rows)
     lib, stream = _lib(), _stream()
-    nb = lib.vi_prefix_attention_workspace_bytes(rows, heads, kv_heads, dim, lanes, groups, max_rows, max_group_rows,
-                                                 max_own, max_prefix)
+    nb = lib.vi_prefix_attention_workspace_bytes(rows, heads, kv_heads, dim, tables.shape[0], groups, max_rows,
+                                                 max_group_rows, max_own, max_prefix)
     ws = workspace(("attention", stream), nb, q.device)
     check(lib.vi_prefix_attention(
-        cache, _lane_args(tables, row_offsets, context, rows), heads, _abi.HEAD_ROWS.pack(*qa),
-        1.0 / math.sqrt(dim) if scale is None else scale, groups, go, pl, max_rows, max_group_rows, max_own,
-        max_prefix, None if tree is None else _int_list(tree, torch.int64, "tree", rows), *oa,
+        cache, lanes, heads, _abi.HEAD_ROWS.pack(*qa), 1.0 / math.sqrt(dim) if scale is None else scale, groups, go,
+        pl, max_rows, max_group_rows, max_own, max_prefix,
+        None if tree is None else _int_list(tree, _I64, "tree", rows), *oa,
         None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream), "vi_prefix_attention")
     return out
 
 
 def _map_args(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor | None, page_size: int,
               status: torch.Tensor | None) -> bytes:
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1 or not tables.is_cuda:
-        raise ValueError("tables must be int32 [lanes, pages per lane] with contiguous rows")
-    lanes, width = tables.shape
-    return _abi.PAGE_MAP.pack(_int_list(refs, torch.int32, "refs"), tables.data_ptr(),
-                              0 if lengths is None else _int_list(lengths, torch.int32, "lengths", lanes),
-                              0 if status is None else _int_list(status, torch.int32, "status", 3),
-                              max(tables.stride(0), width), refs.numel(), page_size, lanes, width)
+    address, stride, lanes, width = _table_args(tables)
+    return _abi.PAGE_MAP.pack(_int_list(refs, _I32, "refs"), address,
+                              0 if lengths is None else _int_list(lengths, _I32, "lengths", lanes),
+                              0 if status is None else _int_list(status, _I32, "status", 3), stride, refs.numel(),
+                              page_size, lanes, width)
 
 
 def _pool_args(pool: torch.Tensor, pages: int) -> bytes:
-    if pool.dim() < 4 or not pool.is_contiguous() or not pool.is_cuda or pool.shape[-4] != pages:
+    if pool.dim() < 4 or not pool.is_cuda or not pool.is_contiguous() or pool.shape[-4] != pages:
         raise ValueError("pool must be contiguous [..., pages, kv_heads, page_size, head_dim] device memory")
-    page_bytes = pool.stride(-4) * pool.element_size()
-    return _abi.PAGE_POOL.pack(pool.data_ptr(), page_bytes * pages, page_bytes, pool.numel() // (pool.stride(-4) * pages),
-                               0)
+    elements = pool.stride(-4)
+    page_bytes = elements * pool.element_size()
+    return _abi.PAGE_POOL.pack(pool.data_ptr(), page_bytes * pages, page_bytes, pool.numel() // (elements * pages), 0)
 
 
 def _pair(a: torch.Tensor, b: torch.Tensor, names: tuple[str, str]) -> tuple[int, int, int]:
     n = a.numel()
-    return _int_list(a, torch.int32, names[0]), _int_list(b, torch.int32, names[1], n), n
+    return _int_list(a, _I32, names[0]), _int_list(b, _I32, names[1], n), n
 
 
 def pages_fork(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor,
@@ -223,15 +227,12 @@ def keep_rows(pool: torch.Tensor, tables: torch.Tensor, lanes: torch.Tensor, con
     """Row paths[i, j] (int32 [n, width]) of lanes[i], appended at context[i], moves
     to cache index context[i] + j for j < kept[i], in every plane (vi_keep_rows)."""
     n = lanes.numel()
-    if paths.dtype != torch.int32 or paths.dim() != 2 or paths.shape[0] != n or not paths.is_contiguous() or \
+    if paths.dtype is not _I32 or paths.dim() != 2 or paths.shape[0] != n or not paths.is_contiguous() or \
             not paths.is_cuda:
         raise ValueError("paths must be contiguous int32 [lanes, width] device memory")
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1 or not tables.is_cuda:
-        raise ValueError("tables must be int32 [lanes, pages per lane] with contiguous rows")
+    address, stride, count, width = _table_args(tables)
     pages, kv_heads, page_size, _ = pool.shape[-4:]
     check(_lib().vi_keep_rows(
-        _abi.PAGE_MAP.pack(0, tables.data_ptr(), 0, 0, max(tables.stride(0), tables.shape[1]), pages, page_size,
-                           tables.shape[0], tables.shape[1]),
-        _pool_args(pool, pages), kv_heads, _int_list(lanes, torch.int32, "lanes"),
-        _int_list(context, torch.int32, "context", n), paths.data_ptr(), paths.shape[1],
-        _int_list(kept, torch.int32, "kept", n), n, _stream()), "vi_keep_rows")
+        _abi.PAGE_MAP.pack(0, address, 0, 0, stride, pages, page_size, count, width), _pool_args(pool, pages), kv_heads,
+        _int_list(lanes, _I32, "lanes"), _int_list(context, _I32, "context", n), paths.data_ptr(), paths.shape[1],
+        _int_list(kept, _I32, "kept", n), n, _stream()), "vi_keep_rows")

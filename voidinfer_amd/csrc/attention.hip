@@ -95,7 +95,7 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, v
     const uint32_t at = __builtin_amdgcn_readfirstlane(
         uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to)));
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(at)
-                 : "memory", "m0");
+                 : "memory");
 }
 __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
