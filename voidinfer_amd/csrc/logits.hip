@@ -5,10 +5,9 @@
 // number of occurrences, a bias the last entry that names it: both are rare in a
 // slice, so each thread requests its logits first (they stay in registers),
 // then the workgroup goes over the lane's lists and notes what falls into the
-// slice in LDS: a bitmap of touched tokens and, for these only, a counter and a
-// bias index.  The arrays are never cleared as a whole: a first pass over the lists
-// sets the bits and zeroes the entries it will use, a second adds.  Vectors of
-// eight tokens whose byte of the bitmap is zero go through unread and unrounded.
+// slice in LDS: a bitmap of touched tokens and a counter per token, then, in the
+// same array, the biases' places in their list.  Vectors whose part of a bitmap
+// is zero go through unread and unrounded.
 #include <algorithm>
 
 #include "penalty_state.h"
@@ -30,7 +29,6 @@ struct RuleArgs {
     vi_logit_rules r;
     PenaltyLayout layout;
     uint32_t* row_flags;
-    int count_at, bias_at;   // LDS words: the counters, the bias indices
 };
 
 template <int DT> constexpr uint32_t kMasked = DT == VI_BF16 ? 0xff80ff80u : DT == VI_F16 ? 0xfc00fc00u : 0xff800000u;
@@ -79,15 +77,40 @@ __device__ __forceinline__ float penalize_value(float y, uint32_t count, const v
     return y;
 }
 
+// A list's entries [offsets[at], offsets[at + 1]), dealt out over the threads, kHeld
+// of a thread in flight at once; the first are requested on construction.
+template <int kHeld> struct List {
+    const int32_t* list;
+    int64_t b = 0, e = 0;
+    int held[kHeld];
+
+    __device__ __forceinline__ List(const int32_t* l, const int64_t* offsets, int at) : list(l) {
+        if (list) { b = offsets[at]; e = offsets[at + 1]; }
+        if (b + int(threadIdx.x) < e) request(b + threadIdx.x);
+    }
+    __device__ __forceinline__ void request(int64_t i) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) held[j] = list[min(i + j * kRuleThreads, e - 1)];
+    }
+    template <class F> __device__ __forceinline__ void each(F&& f) {
+        for (int64_t i = b + threadIdx.x; i < e; i += kRuleThreads * kHeld) {
+            if (e - b > kRuleThreads * kHeld) request(i);   // (more than was held)
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                if (i + j * kRuleThreads < e) f(held[j], uint32_t(i + j * kRuleThreads - b));
+        }
+    }
+};
+
 template <int DT>
-__global__ __launch_bounds__(kRuleThreads) void rules_kernel(RuleArgs a) {
+__global__ __launch_bounds__(kRuleThreads, 8) void rules_kernel(RuleArgs a) {
     constexpr int kPer = Elem<DT>::kPerVec, kVecs = kRuleSlice / (kRuleThreads * kPer);
+    constexpr uint32_t kAll = (1u << kPer) - 1u;
     using Bits = typename Elem<DT>::Bits;
-    extern __shared__ uint32_t lds[];
+    extern __shared__ __align__(16) uint32_t lds[];
     uint32_t* const seen = lds;                   // tokens with an occurrence
     uint32_t* const biased = lds + kRuleWords;    // tokens with a bias
-    uint32_t* const count = lds + a.count_at;
-    uint32_t* const bias = lds + a.bias_at;
+    uint32_t* const value = lds + 2 * kRuleWords; // [kRuleSlice] occurrences, then places in the bias list
 
     const int tid = threadIdx.x, row = int(blockIdx.x / unsigned(a.slices)), slice = int(blockIdx.x % unsigned(a.slices));
     const int first = slice * kRuleSlice, n = min(kRuleSlice, a.vocabulary - first);
@@ -116,13 +139,18 @@ __global__ __launch_bounds__(kRuleThreads) void rules_kernel(RuleArgs a) {
     const bool biases = !failed && r.bias_ids;
     penalties = penalties && !failed;
 
-    // the thread's logits and mask bits: a masked vector's logits are not read
+    // the first entries of the lane's lists, and below the thread's logits and mask
+    // bits, are requested together: what follows waits for memory once
+    List<8> history(penalties ? r.histories : nullptr, r.history_offsets, lane);
+    List<1> extra(penalties ? r.extra : nullptr, r.extra_offsets, row);
+    List<1> bias(biases ? r.bias_ids : nullptr, r.bias_offsets, lane);
+    // a masked vector's logits are not read
     uint4 v[kVecs];
     uint32_t allowed[kVecs];
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
         const int t = (k * kRuleThreads + tid) * kPer;
-        allowed[k] = failed ? 0u : (1u << kPer) - 1u;
+        allowed[k] = failed ? 0u : kAll;
         if (!failed && mask >= 0 && t < n) {
             const uint32_t w = r.mask_words[int64_t(mask) * r.mask_stride + ((first + t) >> 5)];
             allowed[k] &= w >> (t & 31);
@@ -140,76 +168,83 @@ __global__ __launch_bounds__(kRuleThreads) void rules_kernel(RuleArgs a) {
         }
     }
 
+    float y[kVecs * kPer];   // what the touched logits become
+    uint32_t touched = 0;
     if (penalties || biases) {
         for (int i = tid; i < 2 * kRuleWords; i += kRuleThreads) lds[i] = 0u;
-        __syncthreads();
-        int64_t hb = 0, he = 0, eb = 0, ee = 0, bb = 0, be = 0;
-        if (penalties && r.histories) { hb = r.history_offsets[lane]; he = r.history_offsets[lane + 1]; }
-        if (penalties && r.extra) { eb = r.extra_offsets[row]; ee = r.extra_offsets[row + 1]; }
-        if (biases) { bb = r.bias_offsets[lane]; be = r.bias_offsets[lane + 1]; }
-        const uint32_t* const present = state ? reinterpret_cast<const uint32_t*>(state + a.layout.off_b1) : nullptr;
-        const uint2* const table = state ? reinterpret_cast<const uint2*>(state + a.layout.off_hash) : nullptr;
-        const int words = (n + 31) / 32;
+        if (penalties)
+            for (int i = tid * 4; i < kRuleSlice; i += kRuleThreads * 4)
+                *reinterpret_cast<uint4*>(value + i) = make_uint4(0, 0, 0, 0);
         bool bad = false;
-        auto mark = [&](const int32_t* list, int64_t b, int64_t e, uint32_t* bits, uint32_t* value) {
-            for (int64_t i = b + tid; i < e; i += kRuleThreads) {
-                const int t = list[i] - first;
-                bad |= uint32_t(list[i]) >= uint32_t(a.vocabulary);
-                if (uint32_t(t) < uint32_t(n)) {
-                    atomicOr(&bits[t >> 5], 1u << (t & 31));
-                    value[t] = 0u;
+        auto each = [&](auto& list, auto&& f) {
+            list.each([&](int token, uint32_t i) {
+                bad |= uint32_t(token) >= uint32_t(a.vocabulary);
+                if (uint32_t(token - first) < uint32_t(n)) f(token - first, i);
+            });
+        };
+        __syncthreads();
+        if (penalties) {
+            auto count = [&](int t, uint32_t) {
+                atomicAdd(&value[t], 1u);
+                atomicOr(&seen[t >> 5], 1u << (t & 31));
+            };
+            each(history, count);
+            each(extra, count);
+            if (state && tid < (n + 31) / 32) {
+                const uint32_t* const present = reinterpret_cast<const uint32_t*>(state + a.layout.off_b1);
+                const uint2* const table = reinterpret_cast<const uint2*>(state + a.layout.off_hash);
+                const uint32_t word = present[(first >> 5) + tid];
+                if (word) atomicOr(&seen[tid], word);
+                for (uint32_t m = word; m; m &= m - 1u) {
+                    const int t = tid * 32 + __builtin_ctz(m);
+                    atomicAdd(&value[t], hash_count(table, a.layout.shift, a.layout.slots, first + t));
                 }
             }
-        };
-        uint32_t mine = 0u;
-        if (present && tid < words) {
-            mine = present[(first >> 5) + tid];
-            if (mine) atomicOr(&seen[tid], mine);
-            for (uint32_t m = mine; m; m &= m - 1u) count[tid * 32 + __builtin_ctz(m)] = 0u;
-        }
-        mark(r.histories, hb, he, seen, count);
-        mark(r.extra, eb, ee, seen, count);
-        mark(r.bias_ids, bb, be, biased, bias);
-        __syncthreads();
-        for (uint32_t m = mine; m; m &= m - 1u) {
-            const int t = tid * 32 + __builtin_ctz(m);
-            atomicAdd(&count[t], hash_count(table, a.layout.shift, a.layout.slots, first + t));
-        }
-        auto add = [&](const int32_t* list, int64_t b, int64_t e) {
-            for (int64_t i = b + tid; i < e; i += kRuleThreads) {
-                const int t = list[i] - first;
-                if (uint32_t(t) < uint32_t(n)) atomicAdd(&count[t], 1u);
-            }
-        };
-        add(r.histories, hb, he);
-        add(r.extra, eb, ee);
-        for (int64_t i = bb + tid; i < be; i += kRuleThreads) {
-            const int t = r.bias_ids[i] - first;
-            if (uint32_t(t) < uint32_t(n)) atomicMax(&bias[t], uint32_t(i - bb));   // the last entry of a token
-        }
-        if (__syncthreads_or(bad)) flags |= uint32_t(VI_FLAG_BAD_HISTORY);
+            __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kVecs; ++k) {
-            const int t = (k * kRuleThreads + tid) * kPer;
-            if (t >= n) continue;
-            constexpr uint32_t kAll = (1u << kPer) - 1u;
-            const uint32_t s = seen[t >> 5] >> (t & 31) & kAll & allowed[k];
-            const uint32_t b = biased[t >> 5] >> (t & 31) & kAll & allowed[k];
-            if (!(s | b)) continue;
+            for (int k = 0; k < kVecs; ++k) {
+                const int t = (k * kRuleThreads + tid) * kPer;
+                const uint32_t s = t < n ? seen[t >> 5] >> (t & 31) & kAll & allowed[k] : 0u;
+                if (!s) continue;
+                touched |= s << (k * kPer);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                if (!((s | b) >> j & 1u)) continue;
-                float y = Elem<DT>::decode(vec_bits<DT>(v[k], j));
-                if (s >> j & 1u) y = penalize_value(y, count[t + j], p);
-                if (b >> j & 1u) y = y + r.bias_values[bb + bias[t + j]];
-                set_bits<DT>(v[k], j, Elem<DT>::round(y));
+                for (int j = 0; j < kPer; ++j)
+                    if (s >> j & 1u) y[k * kPer + j] = penalize_value(Elem<DT>::decode(vec_bits<DT>(v[k], j)), value[t + j], p);
             }
         }
+        if (biases) {
+            // (the places in the list need no cleared array: those of the tokens that have one)
+            __syncthreads();
+            each(bias, [&](int t, uint32_t) {
+                atomicOr(&biased[t >> 5], 1u << (t & 31));
+                value[t] = 0u;
+            });
+            __syncthreads();
+            each(bias, [&](int t, uint32_t i) { atomicMax(&value[t], i); });   // the last entry of a token
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k) {
+                const int t = (k * kRuleThreads + tid) * kPer;
+                const uint32_t s = t < n ? biased[t >> 5] >> (t & 31) & kAll & allowed[k] : 0u;
+                if (!s) continue;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    if (!(s >> j & 1u)) continue;
+                    const float x = touched >> (k * kPer + j) & 1u ? y[k * kPer + j] : Elem<DT>::decode(vec_bits<DT>(v[k], j));
+                    y[k * kPer + j] = x + r.bias_values[bias.b + value[t + j]];
+                }
+                touched |= s << (k * kPer);
+            }
+        }
+        if (slice == 0 && __syncthreads_or(bad)) flags |= uint32_t(VI_FLAG_BAD_HISTORY);
     }
     if (a.row_flags && slice == 0 && tid == 0) a.row_flags[row] = flags;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
         const int t = (k * kRuleThreads + tid) * kPer;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (touched >> (k * kPer + j) & 1u) set_bits<DT>(v[k], j, Elem<DT>::round(y[k * kPer + j]));
         apply_mask<DT>(v[k], allowed[k]);
         if (t + kPer <= n) {
             store16(out + t, v[k]);
@@ -230,11 +265,8 @@ vi_status launch_rules(const void* logits, int dtype, int rows, int vocabulary, 
     a.rows = rows; a.vocabulary = vocabulary; a.slices = (vocabulary + kRuleSlice - 1) / kRuleSlice;
     a.r = rules; a.row_flags = row_flags;
     if (rules.states) a.layout = penalty_layout(vocabulary, rules.slots);
-    size_t words = 2 * kRuleWords;
-    a.count_at = int(words);
-    if (rules.params && (rules.histories || rules.states || rules.extra)) words += kRuleSlice;
-    a.bias_at = int(words);
-    if (rules.bias_ids) words += kRuleSlice;
+    const bool lists = rules.bias_ids || (rules.params && (rules.histories || rules.states || rules.extra));
+    const size_t words = lists ? 2 * kRuleWords + kRuleSlice : 0;
     const int64_t blocks = int64_t(rows) * a.slices;
     if (blocks > 0x7fffffff) return VI_ERR_UNSUPPORTED;
     auto* kernel = dtype == VI_BF16 ? rules_kernel<VI_BF16> : dtype == VI_F16 ? rules_kernel<VI_F16> : rules_kernel<VI_F32>;
