@@ -35,7 +35,14 @@ struct ScopePlan {
 };
 struct AttnPlan {
     ScopePlan prefix, own;
-    int parts() const { return prefix.splits + own.splits; }
+};
+// Where the join finds a row's parts; written by its lane's first own part.
+struct RowInfo {
+    int32_t lane, group;        // group: -1 without
+    int32_t own_row, group_row; // the row's place in the two scopes
+    int32_t own_parts, group_parts;
+    int32_t lost;               // outside the caller's bounds
+    int32_t reserved;
 };
 
 struct AttnArgs {
@@ -53,8 +60,12 @@ struct AttnArgs {
     int64_t out_row, out_head;
     float* lse;
     AttnPlan plan;
-    float* part_o;         // [parts][rows * heads][head_dim], unnormalised
-    float2* part_ml;       // [parts][rows * heads]: maximum (raw scores), sum (negative: marked)
+    // parts by blocks of 32 queries, the prefixes' blocks first; a block's sums
+    // (unnormalised) as the waves hold them, [head_dim / 8][half][query][4], and per
+    // query the maximum (raw scores) and the sum (negative: marked)
+    float* part_o;
+    float2* part_ml;
+    RowInfo* info;         // [rows]
 };
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -184,6 +195,34 @@ __device__ __forceinline__ int parts_used(const Scope& s, const ScopePlan& p) {
     return int(min(int64_t(p.splits), (s.end - base + p.chunk - 1) / p.chunk));
 }
 
+__device__ __forceinline__ void row_info(const AttnArgs& a, const Scope& own, int lane) {
+    RowInfo r{lane, -1, 0, 0, parts_used(own, a.plan.own), 0, 0, 0};
+    int group_row0 = 0;
+    if (a.groups) {
+        const int g = lane_of_row(a.group_offsets, a.groups, lane);
+        const Scope p = prefix_scope(a, g);
+        if (lane >= a.group_offsets[g] && lane < a.group_offsets[g + 1] && p.end > 0) {
+            r.group = g;
+            r.group_parts = parts_used(p, a.plan.prefix);
+            group_row0 = p.row0;
+        }
+    }
+    for (int i = threadIdx.x; i < own.rows; i += kAttnThreads) {
+        r.own_row = i;
+        r.group_row = own.row0 + i - group_row0;
+        r.lost = i >= a.max_rows || (r.group >= 0 && r.group_row >= a.max_group_rows);
+        if (own.row0 + i < a.lanes.rows) a.info[own.row0 + i] = r;
+    }
+}
+
+// First block of a part: split `split` of scope `which` (of `scopes`), one kv head.
+__device__ __forceinline__ int64_t part_block(const AttnArgs& a, bool is_prefix, int split, int which, int head) {
+    const ScopePlan& p = is_prefix ? a.plan.prefix : a.plan.own;
+    const int64_t before = is_prefix ? 0 : int64_t(a.plan.prefix.splits) * a.groups * a.cache.kv_heads * a.plan.prefix.tiles * a.plan.prefix.waves;
+    const int scopes = is_prefix ? a.groups : a.lanes.lanes;
+    return before + ((int64_t(split) * scopes + which) * a.cache.kv_heads + head) * (p.tiles * p.waves);
+}
+
 template <int D> struct Tile {
     static constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
     static constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
@@ -196,7 +235,7 @@ template <int D> using Tiles = unsigned char[2][2][kTileBytes];   // [stage][key
 // waves hold 32 queries each; the others share the tile's blocks of keys with them.
 template <int DT, int D, int kWaves>
 __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, const Scope& s, bool is_prefix,
-                                            int head, int queries, int m0, int64_t k0, int64_t k1, int64_t part) {
+                                            int head, int queries, int m0, int64_t k0, int64_t k1, int64_t block) {
     using T = Tile<D>;
     constexpr int kKeys = T::kKeys, kBlocks = T::kBlocks, kChunks = T::kChunks, kRowsPerLoad = T::kRowsPerLoad;
     constexpr int kLoads = T::kLoads, kSteps = T::kSteps, kOuts = T::kOuts;
@@ -455,15 +494,14 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
     if (!live || ki > 0) return;
     sum = halves_sum(sum);
     marked = halves_max(marked ? 1.0f : 0.0f) > 0.0f;
-    const int64_t at = part * (int64_t(a.lanes.rows) * a.heads) + int64_t(row) * a.heads + qhead;
-    if (half == 0) a.part_ml[at] = make_float2(top, marked ? -sum : sum);
-    float* const o = a.part_o + at * D + 4 * half;
+    block += m0 / 32 + qi;
+    if (half == 0) a.part_ml[block * 32 + col] = make_float2(top, marked ? -sum : sum);
+    float4* const o = reinterpret_cast<float4*>(a.part_o + block * (32 * D)) + lane;
 #pragma unroll
     for (int d = 0; d < kOuts; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(o + d * 32 + 2 * e) =
-                make_float4(acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]);
+        for (int e = 0; e < 4; ++e)
+            o[(d * 4 + e) * kWave] = make_float4(acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]);
 }
 
 template <int DT, int D>
@@ -484,13 +522,14 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(
     const Scope s = is_prefix ? prefix_scope(a, which) : own_scope(a, which);
     const int queries = min(s.rows, is_prefix ? a.max_group_rows : a.max_rows) * (a.heads / kv_heads);
     const int m0 = tile * 32 * plan.waves;
+    if (!is_prefix && head == 0 && tile == 0 && split == 0) row_info(a, s, which);
     int64_t k0, k1;
     part_range(s, plan, split, &k0, &k1);
     if (m0 >= queries || k0 >= k1) return;
-    const int64_t part = is_prefix ? split : a.plan.prefix.splits + split;
-    if (plan.waves == 4) attend_part<DT, D, 4>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
-    else if (plan.waves == 2) attend_part<DT, D, 2>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
-    else attend_part<DT, D, 1>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, part);
+    const int64_t block = part_block(a, is_prefix, split, which, head);
+    if (plan.waves == 4) attend_part<DT, D, 4>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
+    else if (plan.waves == 2) attend_part<DT, D, 2>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
+    else attend_part<DT, D, 1>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
 }
 
 // The infinities and NaN among the values of a marked part that the row sees, in
@@ -517,51 +556,57 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
     return make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// The parts of every (row, head) joined.  D / 4 threads a pair.
+// The parts of every (row, head) joined.  Thread by thread the query heads of one kv
+// head and row, then the places, four each: neighbours read neighbouring queries
+// of a part's block.
 template <int DT, int D>
 __global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
-    constexpr int kPer = D / 4;
-    const int64_t at = int64_t(blockIdx.x) * (kAttnThreads / kPer) + threadIdx.x / kPer;
-    const int d = threadIdx.x % kPer * 4;
-    const int64_t pairs = int64_t(a.lanes.rows) * a.heads;
-    const int row = int(at / a.heads), head = int(at % a.heads);
-    if (at >= pairs || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
-    const int lane = lane_of_row(a.lanes.row_offsets, a.lanes.lanes, row);
-    const Scope own = own_scope(a, lane);
-    bool bad = row - own.row0 >= a.max_rows;
-    int used[2] = {0, 0};
-    Scope shared{};
-    if (a.groups) {
-        const int g = lane_of_row(a.group_offsets, a.groups, lane);
-        if (lane >= a.group_offsets[g] && lane < a.group_offsets[g + 1]) {
-            shared = prefix_scope(a, g);
-            if (shared.end > 0) {
-                bad |= row - shared.row0 >= a.max_group_rows;
-                used[0] = parts_used(shared, a.plan.prefix);
-            }
-        }
-    }
-    used[1] = parts_used(own, a.plan.own);
+    constexpr int kQuads = D / 4;
+    const int per_kv = a.heads / a.cache.kv_heads;
+    const int64_t t = int64_t(blockIdx.x) * kAttnThreads + threadIdx.x;
+    const int64_t span = int64_t(per_kv) * kQuads;   // threads of a (row, kv head)
+    const int row = int(t / (span * a.cache.kv_heads));
+    if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
+    const int kv = int(t / span % a.cache.kv_heads), in = int(t % span);
+    const int g = in % per_kv, d = in / per_kv * 4, head = kv * per_kv + g;
+    const RowInfo r = a.info[row];
     float top = -kInfF, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-    if (!bad) {
-        for (int k = 0; k < 2; ++k) {
-            const int64_t first = k ? a.plan.prefix.splits : 0;
-            for (int i = 0; i < used[k]; ++i) {
-                float2 ml = a.part_ml[(first + i) * pairs + at];
-                float4 v = *reinterpret_cast<const float4*>(a.part_o + ((first + i) * pairs + at) * D + d);
-                if (__builtin_signbit(ml.y)) {
-                    ml.y = -ml.y;
-                    const float4 x = no_numbers<DT>(a, k ? own : shared, k ? a.plan.own : a.plan.prefix, i, row, head, d, !k);
-                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    if (!r.lost) {
+        for (int k = 0; k < 2; ++k) {   // the group's parts, then the lane's own
+            const int parts = k ? r.own_parts : r.group_parts, which = k ? r.lane : r.group;
+            if (parts == 0) continue;
+            const int m = (k ? r.own_row : r.group_row) * per_kv + g;
+            const ScopePlan& plan = k ? a.plan.own : a.plan.prefix;
+            const int64_t first = part_block(a, !k, 0, which, kv) + m / 32;
+            const int64_t step = part_block(a, !k, 1, which, kv) + m / 32 - first;
+            const int at = (d / 8 * 2 + (d / 4 & 1)) * 32 + m % 32;   // of a block, in float4
+            for (int i0 = 0; i0 < parts; i0 += 4) {   // four parts' loads in flight
+                float2 ml[4];
+                float4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t block = first + min(i0 + j, parts - 1) * step;
+                    ml[j] = a.part_ml[block * 32 + m % 32];
+                    v[j] = reinterpret_cast<const float4*>(a.part_o + block * (32 * D))[at];
                 }
-                if (ml.x == -kInfF && ml.y == 0.0f) continue;   // it saw nothing
-                const float next = fmaxf(top, ml.x);
-                const float x = rescale(top, next, a.scale2), y = rescale(ml.x, next, a.scale2);
-                top = next;
-                sum = sum * x + ml.y * y;
-                o.x = o.x * x + v.x * y; o.y = o.y * x + v.y * y;
-                o.z = o.z * x + v.z * y; o.w = o.w * x + v.w * y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (i0 + j >= parts) break;
+                    if (__builtin_signbit(ml[j].y)) {
+                        ml[j].y = -ml[j].y;
+                        const Scope s = k ? own_scope(a, which) : prefix_scope(a, which);
+                        const float4 x = no_numbers<DT>(a, s, plan, i0 + j, row, head, d, !k);
+                        v[j].x += x.x; v[j].y += x.y; v[j].z += x.z; v[j].w += x.w;
+                    }
+                    if (ml[j].x == -kInfF && ml[j].y == 0.0f) continue;   // it saw nothing
+                    const float next = fmaxf(top, ml[j].x);
+                    const float x = rescale(top, next, a.scale2), y = rescale(ml[j].x, next, a.scale2);
+                    top = next;
+                    sum = sum * x + ml[j].y * y;
+                    o.x = o.x * x + v[j].x * y; o.y = o.y * x + v[j].y * y;
+                    o.z = o.z * x + v[j].z * y; o.w = o.w * x + v[j].w * y;
+                }
             }
         }
     } else {
@@ -574,7 +619,7 @@ __global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
     w.x = Elem<DT>::round(o.x * inv) | Elem<DT>::round(o.y * inv) << 16;
     w.y = Elem<DT>::round(o.z * inv) | Elem<DT>::round(o.w * inv) << 16;
     *reinterpret_cast<uint2*>(out) = w;
-    if (a.lse && d == 0) a.lse[at] = empty ? -kInfF : (top * a.scale2 + log2f(sum)) * (1.0f / kLog2e);
+    if (a.lse && d == 0) a.lse[int64_t(row) * a.heads + head] = empty ? -kInfF : (top * a.scale2 + log2f(sum)) * (1.0f / kLog2e);
 }
 
 ScopePlan scope_plan(int64_t queries) {
@@ -583,8 +628,7 @@ ScopePlan scope_plan(int64_t queries) {
     p.tiles = int((queries + 32 * p.waves - 1) / (32 * p.waves));
     return p;
 }
-// How the work is cut: chunks of one length, so that about two workgroups a CU
-// have one each, but none shorter than two tiles of the keys.
+// How the work is cut.
 AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int groups, int max_rows, int max_group_rows,
                         int64_t max_own, int64_t max_prefix) {
     AttnPlan p{};
@@ -593,19 +637,42 @@ AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int gr
     p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv);
     const int64_t own_items = int64_t(lanes) * kv_heads * p.own.tiles;
     const int64_t prefix_items = int64_t(groups) * kv_heads * p.prefix.tiles;
-    const int64_t work = own_items * max_own + prefix_items * max_prefix;
-    int64_t chunk = std::max<int64_t>(work / 512, 2 * tile);
-    chunk = int64_t(align_up(size_t(chunk), size_t(tile)));
-    p.own.chunk = p.prefix.chunk = int(std::min<int64_t>(chunk, 1 << 30));
-    p.own.splits = int(std::clamp<int64_t>((max_own + chunk - 1) / chunk, 1, 128));
-    p.prefix.splits = groups ? int(std::clamp<int64_t>((max_prefix + chunk - 1) / chunk, 1, 128)) : 0;
+    // Chunks of about one length: of some lengths, the one that ends first if every
+    // round of workgroups over the CUs takes its chunk and four tiles' time besides
+    // (the start, the parts' way to memory), and a last round is half idle.
+    const double slots = double(device_cus()) * (head_dim == 256 ? 1 : 2);
+    const int64_t longest = std::max<int64_t>(std::max(max_own, max_prefix), 1);
+    auto splits = [](int64_t keys, int64_t chunk) { return std::clamp<int64_t>((keys + chunk - 1) / chunk, 1, 128); };
+    double least = 0.0;
+    int64_t best = 0;
+    for (int64_t chunk = 2 * tile;; chunk += std::max<int64_t>(tile, chunk / 8 / tile * tile)) {
+        const double items = double(own_items * splits(max_own, chunk) +
+                                    (groups ? prefix_items * splits(max_prefix, chunk) : 0));
+        const double time = (items <= slots ? 1.0 : items / slots + 0.5) * double(std::min(chunk, longest) + 4 * tile);
+        if (best == 0 || time < least) { least = time; best = chunk; }
+        if (chunk >= longest || chunk > (1 << 28)) break;
+    }
+    // ... and a scope's chunks alike
+    auto cut = [&](ScopePlan& scope, int64_t keys) {
+        scope.splits = int(splits(keys, best));
+        const int64_t each = (std::max<int64_t>(keys, 1) + scope.splits - 1) / scope.splits;
+        scope.chunk = int(std::min<int64_t>(align_up(size_t(each), size_t(tile)), 1 << 30));
+    };
+    cut(p.own, max_own);
+    if (groups) cut(p.prefix, max_prefix);
     return p;
+}
+// Blocks of 32 queries that all parts take.
+size_t attention_blocks(const AttnPlan& p, int kv_heads, int lanes, int groups) {
+    return size_t(kv_heads) * (size_t(p.own.splits) * lanes * p.own.tiles * p.own.waves +
+                               size_t(p.prefix.splits) * groups * p.prefix.tiles * p.prefix.waves);
 }
 
 template <int DT, int D> void launch_dim(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(kAttnThreads), 0, stream, a);
-    const int64_t pairs = int64_t(a.lanes.rows) * a.heads, per = kAttnThreads / (D / 4);
-    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((pairs + per - 1) / per)), dim3(kAttnThreads), 0, stream, a);
+    const int64_t threads = int64_t(a.lanes.rows) * a.heads * (D / 4);
+    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((threads + kAttnThreads - 1) / kAttnThreads)),
+                       dim3(kAttnThreads), 0, stream, a);
 }
 template <int DT> void launch_type(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     switch (a.cache.head_dim) {
@@ -621,8 +688,9 @@ size_t attention_workspace(int rows, int heads, int kv_heads, int head_dim, int 
                            int max_group_rows, int64_t max_own, int64_t max_prefix) {
     const AttnPlan p = attention_plan(heads, kv_heads, head_dim, lanes, groups, max_rows, max_group_rows, max_own,
                                       max_prefix);
-    const size_t pairs = size_t(rows) * heads * p.parts();
-    return align_up(pairs * head_dim * 4, 256) + align_up(pairs * 8, 256) + 256;
+    const size_t blocks = attention_blocks(p, kv_heads, lanes, groups);
+    return align_up(blocks * 32 * head_dim * 4, 256) + align_up(blocks * 32 * 8, 256) +
+           align_up(size_t(rows) * sizeof(RowInfo), 256);
 }
 
 vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, int heads, const vi_head_rows& q,
@@ -639,14 +707,16 @@ vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, 
     a.out = out; a.out_row = out_row; a.out_head = out_head; a.lse = lse;
     a.plan = attention_plan(heads, cache.kv_heads, cache.head_dim, lanes.lanes, groups, max_rows, max_group_rows, max_own,
                             max_prefix);
-    const size_t pairs = size_t(lanes.rows) * heads * a.plan.parts();
+    const size_t parts = attention_blocks(a.plan, cache.kv_heads, lanes.lanes, groups);
     Carver c(ws, ws_bytes);
-    a.part_o = c.take<float>(pairs * cache.head_dim);
-    a.part_ml = c.take<float2>(pairs);
+    a.part_o = c.take<float>(parts * 32 * cache.head_dim);
+    a.part_ml = c.take<float2>(parts * 32);
+    a.info = c.take<RowInfo>(size_t(lanes.rows));
     if (!c.ok) return VI_ERR_WORKSPACE;
     const int64_t blocks = (int64_t(groups) * a.plan.prefix.tiles * a.plan.prefix.splits +
                             int64_t(lanes.lanes) * a.plan.own.tiles * a.plan.own.splits) * cache.kv_heads;
-    if (blocks > 0x7fffffff || pairs > 0x7fffffffffull) return VI_ERR_UNSUPPORTED;
+    if (blocks > 0x7fffffff || int64_t(lanes.rows) * heads * (cache.head_dim / 4) > int64_t(0x7fffffff) * kAttnThreads)
+        return VI_ERR_UNSUPPORTED;
     if (cache.dtype == VI_BF16) launch_type<VI_BF16>(a, unsigned(blocks), stream);
     else launch_type<VI_F16>(a, unsigned(blocks), stream);
     return launch_status();
