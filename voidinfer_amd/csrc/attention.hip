@@ -4,7 +4,7 @@
 // Work: a scope is a set of consecutive rows that see the same keys through one
 // table: a group's rows over its prefix, or a lane's rows over the tokens
 // past it.  Its queries are rows x (heads per kv head), and a workgroup takes up
-// to 128 of them over one chunk of the keys for one kv head, in one pass with a
+// to 256 of them over one chunk of the keys for one kv head, in one pass with a
 // running maximum and sum.  The parts' sums meet in a second launch.
 //
 // The products are transposed: S^T = K Q^T (32 keys x 32 queries a matrix
@@ -22,8 +22,9 @@
 namespace vi {
 namespace {
 
-constexpr int kAttnThreads = 256;
-constexpr int kAttnWaves = kAttnThreads / kWave;
+constexpr int kJoinThreads = 256;
+constexpr int kStages = 4;         // tiles in LDS: one at work, three on their way
+constexpr int kPageList = 1024;    // pages of the keys at hand
 constexpr int kTileBytes = 16384;  // a tile's keys (and its values) in LDS
 constexpr float kLog2e = 1.44269504088896340736f;
 // A running maximum is raised (and the sums rescaled) only once a score exceeds
@@ -97,18 +98,19 @@ template <int DT> __device__ __forceinline__ s16x8_t pack8(const float* p) {
     }
 }
 
-// 16 bytes a lane from base + offset to LDS (base and `to` wave-uniform, lane i's
-// bytes at to + 16 i), without registers in between.  In assembly because the
+// 16 bytes a lane from base + offset to LDS (base and the LDS address `to`
+// wave-uniform, lane i's bytes at to + 16 i), without registers in between.  In assembly because the
 // compiler waits for every such load before any later read of LDS, also of another
 // buffer: the loads of the next tile would not run beside the work on this one.
-// loads_done() waits for the wave's own, a barrier behind it for everyone's.
-__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, void* to) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(
-        uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)to)));
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(at)
+// loads_done() waits for the wave's own (they end in order), a barrier behind it for
+// everyone's.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to)
                  : "memory");
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int kNewer> __device__ __forceinline__ void loads_done() {   // all but the newest kNewer
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kNewer) : "memory");
+}
 
 template <class T> __device__ __forceinline__ __attribute__((address_space(3))) T* lds_ptr(uint32_t at) {
     return (__attribute__((address_space(3))) T*)at;
@@ -149,6 +151,15 @@ __device__ __forceinline__ float halves_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     const uint32_t lo = r[0], hi = r[1];
     return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// To the scheduler: kProducts matrix instructions, kReads reads of LDS behind each.
+template <int kProducts, int kReads> __device__ __forceinline__ void take_turns() {
+    if constexpr (kProducts > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+        take_turns<kProducts - 1, kReads>();
+    }
 }
 
 // The scope of a row range: its rows, keys and table.
@@ -207,7 +218,7 @@ __device__ __forceinline__ void row_info(const AttnArgs& a, const Scope& own, in
             group_row0 = p.row0;
         }
     }
-    for (int i = threadIdx.x; i < own.rows; i += kAttnThreads) {
+    for (int i = threadIdx.x; i < own.rows; i += blockDim.x) {
         r.own_row = i;
         r.group_row = own.row0 + i - group_row0;
         r.lost = i >= a.max_rows || (r.group >= 0 && r.group_row >= a.max_group_rows);
@@ -226,21 +237,26 @@ __device__ __forceinline__ int64_t part_block(const AttnArgs& a, bool is_prefix,
 template <int D> struct Tile {
     static constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
     static constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
-    static constexpr int kLoads = kKeys / kRowsPerLoad / kAttnWaves;           // loads of a wave for a tile's keys
+    // waves of a workgroup: two a SIMD, or with the sums of 256 places one, which has all of its registers
+    static constexpr int kWaves = D == 256 ? 4 : 8;
+    static constexpr int kLoads = kKeys / kRowsPerLoad / kWaves;               // loads of a wave for a tile's keys
     static constexpr int kSteps = D / 16, kOuts = D / 32;
 };
-template <int D> using Tiles = unsigned char[2][2][kTileBytes];   // [stage][keys, values]
+struct AttnLds {
+    unsigned char tiles[kStages][2][kTileBytes];   // [stage][keys, values]
+    int64_t pages[kPageList];
+};
 
 // One item: queries m0 .. of the scope's over keys k0 .. k1.  kWaves of the workgroup's
 // waves hold 32 queries each; the others share the tile's blocks of keys with them.
 template <int DT, int D, int kWaves>
-__device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, const Scope& s, bool is_prefix,
+__device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, const Scope& s, bool is_prefix,
                                             int head, int queries, int m0, int64_t k0, int64_t k1, int64_t block) {
     using T = Tile<D>;
     constexpr int kKeys = T::kKeys, kBlocks = T::kBlocks, kChunks = T::kChunks, kRowsPerLoad = T::kRowsPerLoad;
     constexpr int kLoads = T::kLoads, kSteps = T::kSteps, kOuts = T::kOuts;
-    constexpr int kAlong = kAttnWaves / kWaves < kBlocks ? kAttnWaves / kWaves : kBlocks;   // waves along the keys
-    constexpr int kMine = kBlocks / kAlong, kStep = kMine >= 2 ? 2 : 1;                      // a wave's blocks; at once
+    constexpr int kAlong = T::kWaves / kWaves < kBlocks ? T::kWaves / kWaves : kBlocks;     // waves along the keys
+    constexpr int kMine = kBlocks / kAlong;                                                  // a wave's blocks
 
     const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int col = lane & 31, half = lane >> 5;
@@ -267,7 +283,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
     }
     const uint64_t seen = live && a.tree && !is_prefix ? a.tree[row] : 0;
 
-    const uint32_t tile_at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&tiles));
+    const uint32_t tile_at = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)&lds.tiles));
     // keys: lane (col, half) reads chunk 2 k + half of row col; values: lane i of 16 reads 4 of the
     // 16 places of row i / 4 (rows 4 half .. 4 half + 3, and the same 8 rows on)
     const int sub = lane & 15, value_row = 4 * half + sub / 4;
@@ -285,8 +301,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
     bool marked = false;
 
     // Tiles begin at multiples of 16 tokens, so the rows of one load lie in one page:
-    // its address is uniform, the lane's part of it fixed.  Lane j of a wave looks up
-    // the page of load j, a tile ahead of the load.
+    // its address is uniform, the lane's part of it fixed.
     const int64_t origin = k0 & ~int64_t(15);
     const int total = int((k1 - origin + kKeys - 1) / kKeys);
     const int64_t all_see = min(k1, s.context);
@@ -294,8 +309,8 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
     const int whole = max(int((all_see - origin) / kKeys), first) - first;   // these come first,
     auto tile_of = [&](int i) { return first + i < total ? first + i : 0; };  // then those behind, then the first
     const int32_t* const table = a.lanes.tables + int64_t(s.table) * a.lanes.table_stride;
-    const unsigned char* const keys_at = static_cast<const unsigned char*>(a.cache.keys) + 2 * int64_t(head) * a.cache.head_stride;
-    const unsigned char* const values_at = static_cast<const unsigned char*>(a.cache.values) + 2 * int64_t(head) * a.cache.head_stride;
+    const unsigned char* const keys_at = static_cast<const unsigned char*>(a.cache.keys);
+    const unsigned char* const values_at = static_cast<const unsigned char*>(a.cache.values);
     uint32_t from_lane[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
@@ -303,79 +318,119 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
         from_lane[j] = uint32_t(2 * r * a.cache.token_stride) +
                        (uint32_t((lane % kChunks) ^ swizzle<D>((wave * kLoads + j) * kRowsPerLoad + r)) << 4);
     }
-    auto look_up = [&](int i) {   // (past the end: the last key's page, masked)
-        const int64_t key = origin + int64_t(tile_of(min(i, total - 1))) * kKeys + (wave * kLoads + (lane & (kLoads - 1))) * kRowsPerLoad;
-        const int64_t e = min(key, k1 - 1) >> shift;
-        return e < a.lanes.table_width ? table[e] : -1;
+    // The pages of the keys, a list's length at a time, as the places where their rows of
+    // this head begin, in bytes.  One that is not there is read as page 0; if every row
+    // sees it, every row is NaN, else its keys are.
+    int covered = 0;                  // the list holds the pages of the tiles that come before this one
+    int list_rel = 0, last_rel = 0;   // the origin and the last key, in tokens from the list's first
+    bool lost = false, lost_later = false;
+    auto have_pages = [&](int i) {    // of tile i
+        if (i < covered) return;
+        __syncthreads();
+        const int begins = i == 0 ? 0 : tile_of(i);   // (the first list: from the first tile on)
+        const int64_t e0 = (origin + int64_t(begins) * kKeys) >> shift;
+        int bad = 0;
+        for (int j = tid; j < kPageList; j += T::kWaves * kWave) {
+            const int64_t e = e0 + j;
+            if (e << shift >= k1) break;
+            const int p = e < a.lanes.table_width ? table[e] : -1;
+            const bool ok = uint32_t(p) < uint32_t(a.cache.pages);
+            lds.pages[j] = 2 * (int64_t(ok ? p : 0) * a.cache.page_stride + int64_t(head) * a.cache.head_stride);
+            if (!ok) bad |= (e << shift < s.context ? 1 : 0) | (min((e + 1) << shift, k1) > s.context ? 2 : 0);
+        }
+        lost |= __syncthreads_or(bad & 1) != 0;
+        lost_later |= __syncthreads_or(bad & 2) != 0;
+        list_rel = int(origin - (e0 << shift));
+        last_rel = int(min(k1 - 1 - (e0 << shift), int64_t(0x7fffffff)));
+        const int tiles = ((kPageList << shift) - list_rel) / kKeys;   // up to this one, from `begins`
+        covered = begins == 0 && tiles >= total ? total : begins == 0 && i > 0 ? i + 1 : max(min(tiles, total) - first, i + 1);
     };
-    auto load_tile = [&](int i, int stage, int pages) {
-        const int first_place = int(origin + int64_t(tile_of(i)) * kKeys) & (ps - 1);
+    const uint32_t token_bytes = uint32_t(2 * a.cache.token_stride);   // (a page's rows lie within 4 GiB)
+    auto look_up = [&](int i) {   // lane j: where the page of the wave's load j of tile i begins (past the end: the last key's)
+        const int rel = list_rel + tile_of(i) * kKeys + (wave * kLoads + (lane & (kLoads - 1))) * kRowsPerLoad;
+        return lds.pages[min(rel, last_rel) >> shift];
+    };
+    auto load_tile = [&](int i, int stage, int64_t pages) {
+        const int rel = list_rel + tile_of(i) * kKeys + wave * (kLoads * kRowsPerLoad);
+        const uint32_t to = tile_at + uint32_t(stage) * (2 * kTileBytes) + uint32_t(wave) * (kLoads * kRowsPerLoad * 2 * D);
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
-            const int r0 = (wave * kLoads + j) * kRowsPerLoad;
-            const int page = __builtin_amdgcn_readlane(pages, j);
-            unsigned char* const kt = &tiles[stage][0][r0 * D * 2];
-            unsigned char* const vt = &tiles[stage][1][r0 * D * 2];
-            if (uint32_t(page) < uint32_t(a.cache.pages)) {
-                const int64_t o = 2 * (int64_t(page) * a.cache.page_stride +
-                                       int64_t((first_place + r0) & (ps - 1)) * a.cache.token_stride);
-                load_to_lds(keys_at + o, from_lane[j], kt);
-                load_to_lds(values_at + o, from_lane[j], vt);
-            } else {   // no such page: keys that are NaN, so that rows that see them are
-                reinterpret_cast<uint4*>(kt)[lane] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-                reinterpret_cast<uint4*>(vt)[lane] = make_uint4(0, 0, 0, 0);
-            }
+            const uint64_t o = (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(pages >> 32), j))) << 32 |
+                                uint32_t(__builtin_amdgcn_readlane(int(pages), j))) +
+                               uint32_t((rel + j * kRowsPerLoad) & (ps - 1)) * token_bytes;
+            load_to_lds(keys_at + o, from_lane[j], to + uint32_t(j * kRowsPerLoad * 2 * D));
+            load_to_lds(values_at + o, from_lane[j], to + uint32_t(kTileBytes + j * kRowsPerLoad * 2 * D));
         }
     };
 
-    // One block or two of 32 keys: scores, weights, values.  Where rows do not see
-    // every key (kMasked): of the tile's keys there are those from `begin` on and below
-    // `end`, and every row sees those below `known`.
-    auto attend = [&]<int kN, bool kMasked>(int stage, int b0, int begin, int end, int known) {
-        // LDS addresses of the lane's first key chunk and of its first values; chunk 2 k + half
-        // and block d of 32 places are these with bits flipped.  (Kept from the optimiser,
-        // which would hold all of them in registers through the loop.)
-        uint32_t key_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + key_lane;
-        uint32_t value_at = tile_at + uint32_t(stage) * (2 * kTileBytes) + kTileBytes + value_lane;
-        asm volatile("" : "+v"(key_at), "+v"(value_at));
-        f32x16_t sc[kN];
+    // A tile's work on the wave's blocks ki, ki + kAlong, ...: the scores, their weights, the
+    // values.  LDS addresses: chunk 2 k + half and block d of 32 places are the lane's first
+    // key chunk and first values with bits flipped.  (Kept from the optimiser, which would
+    // hold all of them in registers through the loop.)
+    auto key_ptr = [&](int stage, int b) {
+        uint32_t at = tile_at + uint32_t(stage) * (2 * kTileBytes) + key_lane + uint32_t(b) * (64 * D);
+        asm volatile("" : "+v"(at));
+        return at;
+    };
+    auto value_ptr = [&](int stage, int b) {
+        uint32_t at = tile_at + uint32_t(stage) * (2 * kTileBytes) + kTileBytes + value_lane + uint32_t(b) * (64 * D);
+        asm volatile("" : "+v"(at));
+        return at;
+    };
+    auto key_fragment = [&](uint32_t key_at, int n, int k) {   // step k of block n (known to the compiler)
+        return *(lds_ptr<s16x8_t>(key_at ^ (k << 5)) + n * kAlong * (4 * D));
+    };
+    auto value_fragment = [&](uint32_t value_at, int n, int kb, int d) {   // places 32 d .. of keys 16 kb .. of block n
+        const int o = (n * kAlong * 32 + kb * 16) * (D / 4);   // in 8 bytes
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>(value_at ^ (d << 6)) + o);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>(value_at ^ (d << 6) ^ kValueFlip) + o + 2 * D);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // Scores of one tile (stages below kKeyStages), then the values of another: in each stage
+    // kTurns products take turns with the reads of the next stage's fragments, so that the
+    // wave's reads go through LDS while its products run.  (Left to itself the compiler puts
+    // each product behind its own fragment's read and waits for LDS every time.)
+    constexpr int kTurns = kOuts < 4 ? kOuts : 4;
+    constexpr int kKeyStages = kMine * kSteps / kTurns, kStagesAll = kKeyStages + 2 * kMine * kOuts / kTurns;
+    auto products = [&]<int kFrom, int kTo>(uint32_t key_at, f32x16_t (&sc)[kMine], uint32_t value_at,
+                                            const s16x8_t (&pf)[kMine][2]) {
+        s16x8_t f[2][kTurns];
+        auto read = [&](int stage, s16x8_t (&to)[kTurns]) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-            s16x8_t kf[kSteps];
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) kf[k] = *lds_ptr<s16x8_t>((key_at ^ (k << 5)) + (b0 + n * kAlong) * (64 * D));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) sc[n] = mfma<DT>(kf[k], qf[k], sc[n]);
-        }
-        uint32_t visible = ~0u;   // bit 8 (i / 4) + i % 4: score i
-        if constexpr (kMasked) {
-            static_assert(kN == 1);
-            const int before = known - b0 * 32;   // of this block
-            uint64_t w;   // the block's keys that the lane's query sees
-            if (is_prefix) w = ~0ull;
-            else if (!a.tree) w = low_bits(before + own_row + 1);
-            else if (before >= 0) w = before >= 32 ? ~0ull : seen << before | low_bits(before);
-            else w = before > -64 ? seen >> -before : 0ull;
-            w &= low_bits(end - b0 * 32) & ~low_bits(begin - b0 * 32);
-            visible = uint32_t(w) >> (4 * half);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float score = sc[0][i];
-                const uint32_t see = bit_mask(visible, 8 * (i / 4) + i % 4);
-                sc[0][i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & see) | (0xff800000u & ~see));
+            for (int j = 0; j < kTurns; ++j) {
+                const int at = (stage < kKeyStages ? stage : stage - kKeyStages) * kTurns + j;
+                to[j] = stage < kKeyStages ? key_fragment(key_at, at / kSteps, at % kSteps)
+                                           : value_fragment(value_at, at / kOuts / 2, at / kOuts % 2, at % kOuts);
             }
+        };
+        read(kFrom, f[kFrom & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int stage = kFrom; stage < kTo; ++stage) {
+            if (stage + 1 < kTo) read(stage + 1, f[(stage + 1) & 1]);
+#pragma unroll
+            for (int j = 0; j < kTurns; ++j) {
+                const int at = (stage < kKeyStages ? stage : stage - kKeyStages) * kTurns + j;
+                if (stage < kKeyStages) {
+                    if (at % kSteps == 0)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[at / kSteps][i] = 0.0f;
+                    sc[at / kSteps] = mfma<DT>(f[stage & 1][j], qf[at % kSteps], sc[at / kSteps]);
+                } else {
+                    acc[at % kOuts] = mfma<DT>(f[stage & 1][j], pf[at / kOuts / 2][at / kOuts % 2], acc[at % kOuts]);
+                }
+            }
+            if (stage + 1 < kKeyStages) take_turns<kTurns, 1>();
+            else take_turns<kTurns, 2>();
+            __builtin_amdgcn_sched_barrier(0);
         }
-        float tile_top = -kInfF;
-#pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tile_top = fmaxf(tile_top, sc[n][i]);
-        tile_top = halves_max(tile_top);
-        const bool raise = (tile_top - top) * a.scale2 > kSlack || top == -kInfF;
+    };
+    // The running maximum takes the scores' in; returns what the weights' exponents subtract.
+    auto raise_top = [&](float most) {
+        most = halves_max(most);
+        const bool raise = (most - top) * a.scale2 > kSlack || top == -kInfF;
         if (ballot(raise)) {
-            const float next = raise ? fmaxf(top, tile_top) : top;
+            const float next = raise ? fmaxf(top, most) : top;
             const float shrink = rescale(top, next, a.scale2);
             sum *= shrink;
 #pragma unroll
@@ -384,86 +439,174 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
                 for (int i = 0; i < 16; ++i) acc[d][i] *= shrink;
             top = next;
         }
-        const float offset = top == -kInfF ? 0.0f : top * a.scale2;
-        s16x8_t pf[kN][2];
+        return top == -kInfF ? 0.0f : top * a.scale2;
+    };
+    auto weights = [&](f32x16_t (&sc)[kMine], s16x8_t (&pf)[kMine][2]) {
+        float most = -kInfF;
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
+        for (int n = 0; n < kMine; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, sc[n][i]);
+        const float offset = raise_top(most);
+#pragma unroll
+        for (int n = 0; n < kMine; ++n) {
             float p[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], a.scale2, -offset));
-                if constexpr (kMasked)
-                    p[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p[i]) &
-                                                         bit_mask(visible, 8 * (i / 4) + i % 4));
                 sum += p[i];
             }
             pf[n][0] = pack8<DT>(p);
             pf[n][1] = pack8<DT>(p + 8);
         }
-        // values that are no numbers must reach the rows that see them, and no others (0 x Inf is
-        // NaN): they count as 0 here, and the part is marked for the join
-        bool dirty = false;
-        if constexpr (kMasked) {
-            const uint4* const v = reinterpret_cast<const uint4*>(&tiles[stage][1][b0 * 64 * D]);
-            bool any = false, there = false;
-            for (int i = lane; i < 32 * kChunks; i += kWave) {
-                const bool no_number = any_nonfinite<DT>(v[i]);
-                const int key = b0 * 32 + i / kChunks;
-                any |= no_number;
-                there |= no_number && key >= begin && key < end;
-            }
-            dirty = ballot(any);
-            marked |= ballot(there) != 0;
-        }
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const uint32_t o = uint32_t((b0 + n * kAlong) * 32 + kb * 16) * (2 * D);
-                s16x8_t vf[kOuts];
-#pragma unroll
-                for (int d = 0; d < kOuts; ++d) {
-                    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((value_at ^ (d << 6)) + o));
-                    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        lds_ptr<s16x4_t>((value_at ^ (d << 6) ^ kValueFlip) + 16 * D + o));
-                    vf[d] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if (kMasked && dirty) vf[d] = finite_or_zero<DT>(vf[d]);
-                }
-#pragma unroll
-                for (int d = 0; d < kOuts; ++d) acc[d] = mfma<DT>(vf[d], pf[n][kb], acc[d]);
-            }
-        }
     };
 
-    int pages = look_up(0), stage = 0, i = 0;
-    load_tile(0, 0, pages);
-    pages = look_up(1);
-    auto arrive = [&] {
-        loads_done();      // this wave's part of the tile has arrived
-        __syncthreads();   // everyone's has, and the other stage is no longer read
-        if (i + 1 < total) load_tile(i + 1, stage ^ 1, pages);
-        pages = look_up(i + 2);
-    };
-    // (two loops: each has its own registers)
-    for (; i < whole; ++i, stage ^= 1) {
-        arrive();
-        if (!active) continue;
+    // Where rows do not see every key of a tile (block b of it): there are the tile's
+    // keys from `begin` on and below `end`, and every row sees those below `known`.
+    auto attend_masked = [&](int stage, int b, int64_t at, int begin, int end, int known) {
+        f32x16_t sc;
 #pragma unroll
-        for (int b = 0; b < kMine; b += kStep) attend.template operator()<kStep, false>(stage, ki + b * kAlong, 0, 0, 0);
+        for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+        const uint32_t key_at = key_ptr(stage, b);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) sc = mfma<DT>(key_fragment(key_at, 0, k), qf[k], sc);
+        const int before = known - b * 32;   // of this block
+        uint64_t w;   // the block's keys that the lane's query sees
+        if (is_prefix) w = ~0ull;
+        else if (!a.tree) w = low_bits(before + own_row + 1);
+        else if (before >= 0) w = before >= 32 ? ~0ull : seen << before | low_bits(before);
+        else w = before > -64 ? seen >> -before : 0ull;
+        w &= low_bits(end - b * 32) & ~low_bits(begin - b * 32);
+        const uint32_t visible = uint32_t(w) >> (4 * half);   // bit 8 (i / 4) + i % 4: score i
+        uint32_t gone = 0;   // keys without a page
+        if (lost_later) {
+            const int64_t key = at + b * 32 + col, e = key >> shift;
+            gone = uint32_t(ballot(key < k1 && !(e < a.lanes.table_width && uint32_t(table[e]) < uint32_t(a.cache.pages))));
+            gone >>= 4 * half;
+        }
+        float most = -kInfF;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float score = sc[i];
+            const uint32_t see = bit_mask(visible, 8 * (i / 4) + i % 4);
+            const uint32_t x = __builtin_bit_cast(uint32_t, score) | (bit_mask(gone, 8 * (i / 4) + i % 4) >> 1);
+            sc[i] = __builtin_bit_cast(float, (x & see) | (0xff800000u & ~see));
+            most = fmaxf(most, sc[i]);
+        }
+        const float offset = raise_top(most);
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scale2, -offset));
+            p[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & bit_mask(visible, 8 * (i / 4) + i % 4));
+            sum += p[i];
+        }
+        const s16x8_t pf[2] = {pack8<DT>(p), pack8<DT>(p + 8)};
+        // values that are no numbers must reach the rows that see them, and no others (0 x Inf is
+        // NaN): they count as 0 here, and the part is marked for the join
+        const uint4* const v = reinterpret_cast<const uint4*>(&lds.tiles[stage][1][b * 64 * D]);
+        bool any = false, there = false;
+        for (int i = lane; i < 32 * kChunks; i += kWave) {
+            const bool no_number = any_nonfinite<DT>(v[i]);
+            const int key = b * 32 + i / kChunks;
+            any |= no_number;
+            there |= no_number && key >= begin && key < end;
+        }
+        const bool dirty = ballot(any) != 0;
+        marked |= ballot(there) != 0;
+        const uint32_t value_at = value_ptr(stage, b);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int d = 0; d < kOuts; ++d) {
+                s16x8_t vf = value_fragment(value_at, 0, kb, d);
+                if (dirty) vf = finite_or_zero<DT>(vf);
+                acc[d] = mfma<DT>(vf, pf[kb], acc[d]);
+            }
+    };
+
+    // Tiles on their way: tile t is in stage t % kStages.
+    constexpr int kTileLoads = 2 * kLoads;
+    int issued = 0;
+    int64_t pages = 0;   // of tile `issued`
+    auto issue_to = [&](int n) {
+        for (; issued < min(n, total); ++issued) {
+            if (issued >= covered) {
+                have_pages(issued);
+                pages = look_up(issued);
+            }
+            load_tile(issued, issued % kStages, pages);
+            if (issued + 1 < covered) pages = look_up(issued + 1);
+        }
+    };
+    auto arrived = [&](int t) {   // this wave's part of tile t
+        const int newer = issued - 1 - t;
+        if (newer >= 3) loads_done<3 * kTileLoads>();
+        else if (newer == 2) loads_done<2 * kTileLoads>();
+        else if (newer == 1) loads_done<kTileLoads>();
+        else loads_done<0>();
+    };
+    issue_to(kStages);
+    int i = 0;
+    if (whole > 0) {
+        f32x16_t sc[kMine];
+        s16x8_t pf[kMine][2];
+        if constexpr (T::kWaves == 8) {
+            // The two waves of a SIMD in turn: while one's products run (scores of tile t, values of
+            // t - 1) the other takes the weights of its scores.  Phase p: waves 0 .. 3 have
+            // products t at p = 2 t and weights t at 2 t + 1, waves 4 .. 7 one phase later.  A
+            // barrier ends each phase; tile t has arrived by the end of phase 2 t - 1, and its
+            // stage is free from phase 2 t + 4 on.
+            const int late = wave >> 2;
+            arrived(0);
+            __syncthreads();
+            if (late) __syncthreads();
+            if (active) products.template operator()<0, kKeyStages>(key_ptr(0, ki), sc, 0, pf);
+            for (;;) {
+                if (late && i + 1 < whole) arrived(i + 1);
+                __syncthreads();
+                if (late) issue_to(i + 4);
+                if (active) weights(sc, pf);
+                if (!late && i + 1 < whole) arrived(i + 1);
+                __syncthreads();
+                if (!late) issue_to(i + 4);
+                if (++i == whole) break;
+                if (active) {
+                    __builtin_amdgcn_s_setprio(1);
+                    products.template operator()<0, kStagesAll>(key_ptr(i % kStages, ki), sc, value_ptr((i - 1) % kStages, ki), pf);
+                    __builtin_amdgcn_s_setprio(0);
+                }
+            }
+            if (active) products.template operator()<kKeyStages, kStagesAll>(0, sc, value_ptr((i - 1) % kStages, ki), pf);
+            __syncthreads();
+            if (!late) __syncthreads();
+        } else {
+            for (; i < whole; ++i) {
+                arrived(i);
+                __syncthreads();
+                issue_to(i + kStages);
+                if (!active) continue;
+                products.template operator()<0, kKeyStages>(key_ptr(i % kStages, ki), sc, 0, pf);
+                weights(sc, pf);
+                products.template operator()<kKeyStages, kStagesAll>(0, sc, value_ptr(i % kStages, ki), pf);
+            }
+        }
     }
-    for (; i < total; ++i, stage ^= 1) {
-        arrive();
+    for (; i < total; ++i) {
+        arrived(i);
+        __syncthreads();   // everyone's part; the tile before is no longer read
+        issue_to(i + kStages);
         if (!active) continue;
         const int64_t at = origin + int64_t(tile_of(i)) * kKeys;
         const int begin = int(max(k0 - at, int64_t(0))), end = int(min(k1 - at, int64_t(kKeys)));
         const int known = int(max(min(s.context - at, int64_t(kKeys)), int64_t(-(1 << 30))));
-        for (int b = 0; b < kMine; ++b) attend.template operator()<1, true>(stage, ki + b * kAlong, begin, end, known);
+        for (int b = 0; b < kMine; ++b) attend_masked(i % kStages, ki + b * kAlong, at, begin, end, known);
     }
 
     // the waves that shared queries join
     if constexpr (kAlong > 1) {
         __syncthreads();
-        float* const mem = reinterpret_cast<float*>(tiles);
+        float* const mem = reinterpret_cast<float*>(lds.tiles);
         constexpr int kPer = kOuts * 16 + 2;   // floats a lane leaves
         if (active && ki > 0) {
             float* const slot = mem + (wave - kWaves) * kPer * kWave + lane;
@@ -492,7 +635,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
         }
     }
     if (!live || ki > 0) return;
-    sum = halves_sum(sum);
+    sum = lost ? __builtin_nanf("") : halves_sum(sum);
     marked = halves_max(marked ? 1.0f : 0.0f) > 0.0f;
     block += m0 / 32 + qi;
     if (half == 0) a.part_ml[block * 32 + col] = make_float2(top, marked ? -sum : sum);
@@ -505,8 +648,8 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, Tiles<D>& tiles, 
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
-    __shared__ __align__(1024) Tiles<D> tiles;
+__global__ __launch_bounds__(Tile<D>::kWaves* kWave, Tile<D>::kWaves / 4) void attend_kernel(AttnArgs a) {
+    __shared__ __align__(1024) AttnLds lds;
     // which item: heads fastest, so that one head's tiles stay on one XCD's L2 where heads are a multiple of 8
     const int kv_heads = a.cache.kv_heads;
     const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
@@ -527,9 +670,11 @@ __global__ __launch_bounds__(kAttnThreads, D == 256 ? 1 : 2) void attend_kernel(
     part_range(s, plan, split, &k0, &k1);
     if (m0 >= queries || k0 >= k1) return;
     const int64_t block = part_block(a, is_prefix, split, which, head);
-    if (plan.waves == 4) attend_part<DT, D, 4>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
-    else if (plan.waves == 2) attend_part<DT, D, 2>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
-    else attend_part<DT, D, 1>(a, tiles, s, is_prefix, head, queries, m0, k0, k1, block);
+    if constexpr (Tile<D>::kWaves == 8)
+        if (plan.waves == 8) return attend_part<DT, D, 8>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
+    if (plan.waves == 4) attend_part<DT, D, 4>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
+    else if (plan.waves == 2) attend_part<DT, D, 2>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
+    else attend_part<DT, D, 1>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
 }
 
 // The infinities and NaN among the values of a marked part that the row sees, in
@@ -560,10 +705,10 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
 // head and row, then the places, four each: neighbours read neighbouring queries
 // of a part's block.
 template <int DT, int D>
-__global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     constexpr int kQuads = D / 4;
     const int per_kv = a.heads / a.cache.kv_heads;
-    const int64_t t = int64_t(blockIdx.x) * kAttnThreads + threadIdx.x;
+    const int64_t t = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x;
     const int64_t span = int64_t(per_kv) * kQuads;   // threads of a (row, kv head)
     const int row = int(t / (span * a.cache.kv_heads));
     if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
@@ -622,9 +767,9 @@ __global__ __launch_bounds__(kAttnThreads) void join_kernel(AttnArgs a) {
     if (a.lse && d == 0) a.lse[int64_t(row) * a.heads + head] = empty ? -kInfF : (top * a.scale2 + log2f(sum)) * (1.0f / kLog2e);
 }
 
-ScopePlan scope_plan(int64_t queries) {
+ScopePlan scope_plan(int64_t queries, int most_waves) {
     ScopePlan p{};
-    p.waves = queries <= 32 ? 1 : queries <= 64 ? 2 : 4;
+    for (p.waves = 1; p.waves < most_waves && queries > 32 * p.waves;) p.waves *= 2;
     p.tiles = int((queries + 32 * p.waves - 1) / (32 * p.waves));
     return p;
 }
@@ -633,14 +778,15 @@ AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int gr
                         int64_t max_own, int64_t max_prefix) {
     AttnPlan p{};
     const int per_kv = heads / kv_heads, tile = kTileBytes / (2 * head_dim);
-    p.own = scope_plan(int64_t(max_rows) * per_kv);
-    p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv);
+    const int most_waves = head_dim == 256 ? Tile<256>::kWaves : Tile<128>::kWaves;
+    p.own = scope_plan(int64_t(max_rows) * per_kv, most_waves);
+    p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv, most_waves);
     const int64_t own_items = int64_t(lanes) * kv_heads * p.own.tiles;
     const int64_t prefix_items = int64_t(groups) * kv_heads * p.prefix.tiles;
     // Chunks of about one length: of some lengths, the one that ends first if every
     // round of workgroups over the CUs takes its chunk and four tiles' time besides
     // (the start, the parts' way to memory), and a last round is half idle.
-    const double slots = double(device_cus()) * (head_dim == 256 ? 1 : 2);
+    const double slots = device_cus();
     const int64_t longest = std::max<int64_t>(std::max(max_own, max_prefix), 1);
     auto splits = [](int64_t keys, int64_t chunk) { return std::clamp<int64_t>((keys + chunk - 1) / chunk, 1, 128); };
     double least = 0.0;
@@ -669,10 +815,10 @@ size_t attention_blocks(const AttnPlan& p, int kv_heads, int lanes, int groups) 
 }
 
 template <int DT, int D> void launch_dim(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
-    hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(kAttnThreads), 0, stream, a);
+    hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(Tile<D>::kWaves * kWave), 0, stream, a);
     const int64_t threads = int64_t(a.lanes.rows) * a.heads * (D / 4);
-    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((threads + kAttnThreads - 1) / kAttnThreads)),
-                       dim3(kAttnThreads), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((threads + kJoinThreads - 1) / kJoinThreads)),
+                       dim3(kJoinThreads), 0, stream, a);
 }
 template <int DT> void launch_type(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     switch (a.cache.head_dim) {
@@ -715,7 +861,7 @@ vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, 
     if (!c.ok) return VI_ERR_WORKSPACE;
     const int64_t blocks = (int64_t(groups) * a.plan.prefix.tiles * a.plan.prefix.splits +
                             int64_t(lanes.lanes) * a.plan.own.tiles * a.plan.own.splits) * cache.kv_heads;
-    if (blocks > 0x7fffffff || int64_t(lanes.rows) * heads * (cache.head_dim / 4) > int64_t(0x7fffffff) * kAttnThreads)
+    if (blocks > 0x7fffffff || int64_t(lanes.rows) * heads * (cache.head_dim / 4) > int64_t(0x7fffffff) * kJoinThreads)
         return VI_ERR_UNSUPPORTED;
     if (cache.dtype == VI_BF16) launch_type<VI_BF16>(a, unsigned(blocks), stream);
     else launch_type<VI_F16>(a, unsigned(blocks), stream);
