@@ -4,7 +4,7 @@
 // Work: a scope is a set of consecutive rows that see the same keys through one
 // table: a group's rows over its prefix, or a lane's rows over the tokens
 // past it.  Its queries are rows x (heads per kv head), and a workgroup takes up
-// to 256 of them over one chunk of the keys for one kv head, in one pass with a
+// to 128 of them over one chunk of the keys for one kv head, in one pass with a
 // running maximum and sum.  The parts' sums meet in a second launch.
 //
 // The products are transposed: S^T = K Q^T (32 keys x 32 queries a matrix
@@ -25,7 +25,8 @@ namespace {
 constexpr int kJoinThreads = 256;
 constexpr int kStages = 4;         // tiles in LDS: one at work, three on their way
 constexpr int kPageList = 1024;    // pages of the keys at hand
-constexpr int kTileBytes = 16384;  // a tile's keys (and its values) in LDS
+// us, two workgroups a CU at work: a part besides its keys, a key at 128 queries, a key below
+constexpr double kPartTime = 7.0, kKeyTimeFull = 0.036, kKeyTime = 0.024;
 constexpr float kLog2e = 1.44269504088896340736f;
 // A running maximum is raised (and the sums rescaled) only once a score exceeds
 // it by this many powers of two: weights stay below 2^8, far from fp16's range.
@@ -235,24 +236,28 @@ __device__ __forceinline__ int64_t part_block(const AttnArgs& a, bool is_prefix,
 }
 
 template <int D> struct Tile {
-    static constexpr int kKeys = kTileBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
+    static constexpr int kBytes = D == 256 ? 16384 : 8192;                     // a tile's keys (and its values) in LDS
+    static constexpr int kKeys = kBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
     static constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
-    // waves of a workgroup: two a SIMD, or with the sums of 256 places one, which has all of its registers
-    static constexpr int kWaves = D == 256 ? 4 : 8;
+    static constexpr int kWaves = 4;
     static constexpr int kLoads = kKeys / kRowsPerLoad / kWaves;               // loads of a wave for a tile's keys
     static constexpr int kSteps = D / 16, kOuts = D / 32;
 };
-struct AttnLds {
-    unsigned char tiles[kStages][2][kTileBytes];   // [stage][keys, values]
+// Two workgroups fit a CU (with the sums of 256 places one, whose waves have all of a
+// SIMD's registers), so that one's start, softmax and waits run beside the other's products.
+template <int D> struct AttnLds {
+    unsigned char tiles[kStages][2][Tile<D>::kBytes];   // [stage][keys, values]
     int64_t pages[kPageList];
+    int32_t bad[Tile<D>::kWaves];
 };
 
 // One item: queries m0 .. of the scope's over keys k0 .. k1.  kWaves of the workgroup's
 // waves hold 32 queries each; the others share the tile's blocks of keys with them.
 template <int DT, int D, int kWaves>
-__device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, const Scope& s, bool is_prefix,
+__device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds<D>& lds, const Scope& s, bool is_prefix,
                                             int head, int queries, int m0, int64_t k0, int64_t k1, int64_t block) {
     using T = Tile<D>;
+    constexpr int kTileBytes = T::kBytes;
     constexpr int kKeys = T::kKeys, kBlocks = T::kBlocks, kChunks = T::kChunks, kRowsPerLoad = T::kRowsPerLoad;
     constexpr int kLoads = T::kLoads, kSteps = T::kSteps, kOuts = T::kOuts;
     constexpr int kAlong = T::kWaves / kWaves < kBlocks ? T::kWaves / kWaves : kBlocks;     // waves along the keys
@@ -277,7 +282,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, con
         for (int k = 0; k < kSteps; ++k) {
             uint4 v = make_uint4(0, 0, 0, 0);
             if (live) v = *reinterpret_cast<const uint4*>(q + k * 16 + half * 8);
-            v.x ^= a.flip; v.y ^= a.flip; v.z ^= a.flip; v.w ^= a.flip;
+            if (a.flip) { v.x ^= a.flip; v.y ^= a.flip; v.z ^= a.flip; v.w ^= a.flip; }
             qf[k] = __builtin_bit_cast(s16x8_t, v);
         }
     }
@@ -326,7 +331,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, con
     bool lost = false, lost_later = false;
     auto have_pages = [&](int i) {    // of tile i
         if (i < covered) return;
-        __syncthreads();
+        if (i > 0) __syncthreads();
         const int begins = i == 0 ? 0 : tile_of(i);   // (the first list: from the first tile on)
         const int64_t e0 = (origin + int64_t(begins) * kKeys) >> shift;
         int bad = 0;
@@ -338,8 +343,15 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, con
             lds.pages[j] = 2 * (int64_t(ok ? p : 0) * a.cache.page_stride + int64_t(head) * a.cache.head_stride);
             if (!ok) bad |= (e << shift < s.context ? 1 : 0) | (min((e + 1) << shift, k1) > s.context ? 2 : 0);
         }
-        lost |= __syncthreads_or(bad & 1) != 0;
-        lost_later |= __syncthreads_or(bad & 2) != 0;
+        const int any = (ballot(bad & 1) ? 1 : 0) | (ballot(bad & 2) ? 2 : 0);
+        if (lane == 0) lds.bad[wave] = any;
+        __syncthreads();
+        bad = 0;
+#pragma unroll
+        for (int w = 0; w < T::kWaves; ++w) bad |= lds.bad[w];
+        bad = __builtin_amdgcn_readfirstlane(bad);
+        lost |= (bad & 1) != 0;
+        lost_later |= (bad & 2) != 0;
         list_rel = int(origin - (e0 << shift));
         last_rel = int(min(k1 - 1 - (e0 << shift), int64_t(0x7fffffff)));
         const int tiles = ((kPageList << shift) - list_rel) / kKeys;   // up to this one, from `begins`
@@ -551,45 +563,14 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, con
     if (whole > 0) {
         f32x16_t sc[kMine];
         s16x8_t pf[kMine][2];
-        if constexpr (T::kWaves == 8) {
-            // The two waves of a SIMD in turn: while one's products run (scores of tile t, values of
-            // t - 1) the other takes the weights of its scores.  Phase p: waves 0 .. 3 have
-            // products t at p = 2 t and weights t at 2 t + 1, waves 4 .. 7 one phase later.  A
-            // barrier ends each phase; tile t has arrived by the end of phase 2 t - 1, and its
-            // stage is free from phase 2 t + 4 on.
-            const int late = wave >> 2;
-            arrived(0);
+        for (; i < whole; ++i) {
+            arrived(i);
             __syncthreads();
-            if (late) __syncthreads();
-            if (active) products.template operator()<0, kKeyStages>(key_ptr(0, ki), sc, 0, pf);
-            for (;;) {
-                if (late && i + 1 < whole) arrived(i + 1);
-                __syncthreads();
-                if (late) issue_to(i + 4);
-                if (active) weights(sc, pf);
-                if (!late && i + 1 < whole) arrived(i + 1);
-                __syncthreads();
-                if (!late) issue_to(i + 4);
-                if (++i == whole) break;
-                if (active) {
-                    __builtin_amdgcn_s_setprio(1);
-                    products.template operator()<0, kStagesAll>(key_ptr(i % kStages, ki), sc, value_ptr((i - 1) % kStages, ki), pf);
-                    __builtin_amdgcn_s_setprio(0);
-                }
-            }
-            if (active) products.template operator()<kKeyStages, kStagesAll>(0, sc, value_ptr((i - 1) % kStages, ki), pf);
-            __syncthreads();
-            if (!late) __syncthreads();
-        } else {
-            for (; i < whole; ++i) {
-                arrived(i);
-                __syncthreads();
-                issue_to(i + kStages);
-                if (!active) continue;
-                products.template operator()<0, kKeyStages>(key_ptr(i % kStages, ki), sc, 0, pf);
-                weights(sc, pf);
-                products.template operator()<kKeyStages, kStagesAll>(0, sc, value_ptr(i % kStages, ki), pf);
-            }
+            issue_to(i + kStages);
+            if (!active) continue;
+            products.template operator()<0, kKeyStages>(key_ptr(i % kStages, ki), sc, 0, pf);
+            weights(sc, pf);
+            products.template operator()<kKeyStages, kStagesAll>(0, sc, value_ptr(i % kStages, ki), pf);
         }
     }
     for (; i < total; ++i) {
@@ -648,14 +629,15 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds& lds, con
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(Tile<D>::kWaves* kWave, Tile<D>::kWaves / 4) void attend_kernel(AttnArgs a) {
-    __shared__ __align__(1024) AttnLds lds;
-    // which item: heads fastest, so that one head's tiles stay on one XCD's L2 where heads are a multiple of 8
+__global__ __launch_bounds__(Tile<D>::kWaves* kWave, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
+    __shared__ __align__(1024) AttnLds<D> lds;
+    // Which item: prefixes' (bound by the products) spread evenly among the lanes' own (bound by
+    // memory), so that the CUs are at both at any time; heads fastest.
     const int kv_heads = a.cache.kv_heads;
-    const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
-    int item = blockIdx.x;
-    const bool is_prefix = item < prefix_items;
-    if (!is_prefix) item -= prefix_items;
+    const uint32_t prefix_items = uint32_t(a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits);
+    const int before = int(uint64_t(blockIdx.x) * prefix_items / gridDim.x);
+    const bool is_prefix = int(uint64_t(blockIdx.x + 1) * prefix_items / gridDim.x) > before;
+    int item = is_prefix ? before : int(blockIdx.x) - before;
     const ScopePlan& plan = is_prefix ? a.plan.prefix : a.plan.own;
     const int head = item % kv_heads;
     item /= kv_heads;
@@ -670,8 +652,6 @@ __global__ __launch_bounds__(Tile<D>::kWaves* kWave, Tile<D>::kWaves / 4) void a
     part_range(s, plan, split, &k0, &k1);
     if (m0 >= queries || k0 >= k1) return;
     const int64_t block = part_block(a, is_prefix, split, which, head);
-    if constexpr (Tile<D>::kWaves == 8)
-        if (plan.waves == 8) return attend_part<DT, D, 8>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
     if (plan.waves == 4) attend_part<DT, D, 4>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
     else if (plan.waves == 2) attend_part<DT, D, 2>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
     else attend_part<DT, D, 1>(a, lds, s, is_prefix, head, queries, m0, k0, k1, block);
@@ -706,7 +686,7 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
 // of a part's block.
 template <int DT, int D>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
-    constexpr int kQuads = D / 4;
+    constexpr int kQuads = D / 4, kBatch = 4;
     const int per_kv = a.heads / a.cache.kv_heads;
     const int64_t t = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x;
     const int64_t span = int64_t(per_kv) * kQuads;   // threads of a (row, kv head)
@@ -726,17 +706,17 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
             const int64_t first = part_block(a, !k, 0, which, kv) + m / 32;
             const int64_t step = part_block(a, !k, 1, which, kv) + m / 32 - first;
             const int at = (d / 8 * 2 + (d / 4 & 1)) * 32 + m % 32;   // of a block, in float4
-            for (int i0 = 0; i0 < parts; i0 += 4) {   // four parts' loads in flight
-                float2 ml[4];
-                float4 v[4];
+            for (int i0 = 0; i0 < parts; i0 += kBatch) {   // so many parts' loads in flight
+                float2 ml[kBatch];
+                float4 v[kBatch];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kBatch; ++j) {
                     const int64_t block = first + min(i0 + j, parts - 1) * step;
                     ml[j] = a.part_ml[block * 32 + m % 32];
                     v[j] = reinterpret_cast<const float4*>(a.part_o + block * (32 * D))[at];
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kBatch; ++j) {
                     if (i0 + j >= parts) break;
                     if (__builtin_signbit(ml[j].y)) {
                         ml[j].y = -ml[j].y;
@@ -767,9 +747,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     if (a.lse && d == 0) a.lse[int64_t(row) * a.heads + head] = empty ? -kInfF : (top * a.scale2 + log2f(sum)) * (1.0f / kLog2e);
 }
 
-ScopePlan scope_plan(int64_t queries, int most_waves) {
+ScopePlan scope_plan(int64_t queries) {
     ScopePlan p{};
-    for (p.waves = 1; p.waves < most_waves && queries > 32 * p.waves;) p.waves *= 2;
+    for (p.waves = 1; p.waves < Tile<128>::kWaves && queries > 32 * p.waves;) p.waves *= 2;
     p.tiles = int((queries + 32 * p.waves - 1) / (32 * p.waves));
     return p;
 }
@@ -777,35 +757,40 @@ ScopePlan scope_plan(int64_t queries, int most_waves) {
 AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int groups, int max_rows, int max_group_rows,
                         int64_t max_own, int64_t max_prefix) {
     AttnPlan p{};
-    const int per_kv = heads / kv_heads, tile = kTileBytes / (2 * head_dim);
-    const int most_waves = head_dim == 256 ? Tile<256>::kWaves : Tile<128>::kWaves;
-    p.own = scope_plan(int64_t(max_rows) * per_kv, most_waves);
-    p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv, most_waves);
+    const int per_kv = heads / kv_heads;
+    const int tile = head_dim == 64 ? Tile<64>::kKeys : head_dim == 128 ? Tile<128>::kKeys : Tile<256>::kKeys;
+    p.own = scope_plan(int64_t(max_rows) * per_kv);
+    p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv);
     const int64_t own_items = int64_t(lanes) * kv_heads * p.own.tiles;
     const int64_t prefix_items = int64_t(groups) * kv_heads * p.prefix.tiles;
-    // Chunks of about one length: of some lengths, the one that ends first if every
-    // round of workgroups over the CUs takes its chunk and four tiles' time besides
-    // (the start, the parts' way to memory), and a last round is half idle.
-    const double slots = device_cus();
-    const int64_t longest = std::max<int64_t>(std::max(max_own, max_prefix), 1);
-    auto splits = [](int64_t keys, int64_t chunk) { return std::clamp<int64_t>((keys + chunk - 1) / chunk, 1, 128); };
+    // Of some lengths of time, the one for which the work is done first if every workgroup
+    // gets as many keys as fit it.
+    const double slots = double(device_cus()) * (head_dim == 256 ? 1 : 2);
+    auto key_time = [&](const ScopePlan& scope) { return scope.waves == 4 ? kKeyTimeFull : kKeyTime; };
+    auto splits = [&](const ScopePlan& scope, int64_t keys, double time) {
+        return int64_t(std::clamp(__builtin_ceil(double(keys) * key_time(scope) / (time - kPartTime)), 1.0, 128.0));
+    };
+    auto part_time = [&](const ScopePlan& scope, int64_t keys, int64_t n) {
+        return kPartTime + key_time(scope) * double((keys + n - 1) / n);
+    };
     double least = 0.0;
-    int64_t best = 0;
-    for (int64_t chunk = 2 * tile;; chunk += std::max<int64_t>(tile, chunk / 8 / tile * tile)) {
-        const double items = double(own_items * splits(max_own, chunk) +
-                                    (groups ? prefix_items * splits(max_prefix, chunk) : 0));
-        const double time = (items <= slots ? 1.0 : items / slots + 0.5) * double(std::min(chunk, longest) + 4 * tile);
-        if (best == 0 || time < least) { least = time; best = chunk; }
-        if (chunk >= longest || chunk > (1 << 28)) break;
+    int64_t own_splits = 1, prefix_splits = 1;
+    for (double time = kPartTime + 2.0; time < 2e4; time *= 1.12) {
+        const int64_t n = splits(p.own, max_own, time), m = splits(p.prefix, max_prefix, time);
+        const double own = part_time(p.own, max_own, n), prefix = groups ? part_time(p.prefix, max_prefix, m) : 0.0;
+        const double longest = std::max(own, prefix), items = double(own_items * n) + (groups ? double(prefix_items * m) : 0.0);
+        const double all = (double(own_items * n) * own + (groups ? double(prefix_items * m) * prefix : 0.0)) / slots;
+        const double done = items <= slots ? longest : all + 0.5 * longest;
+        if (least == 0.0 || done < least) { least = done; own_splits = n; prefix_splits = m; }
+        if (n == 1 && m == 1) break;
     }
-    // ... and a scope's chunks alike
-    auto cut = [&](ScopePlan& scope, int64_t keys) {
-        scope.splits = int(splits(keys, best));
+    auto cut = [&](ScopePlan& scope, int64_t keys, int64_t n) {   // into chunks alike
+        scope.splits = int(n);
         const int64_t each = (std::max<int64_t>(keys, 1) + scope.splits - 1) / scope.splits;
         scope.chunk = int(std::min<int64_t>(align_up(size_t(each), size_t(tile)), 1 << 30));
     };
-    cut(p.own, max_own);
-    if (groups) cut(p.prefix, max_prefix);
+    cut(p.own, max_own, own_splits);
+    if (groups) cut(p.prefix, max_prefix, prefix_splits);
     return p;
 }
 // Blocks of 32 queries that all parts take.
