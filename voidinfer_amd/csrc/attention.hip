@@ -23,10 +23,7 @@ namespace vi {
 namespace {
 
 constexpr int kJoinThreads = 256;
-constexpr int kStages = 4;         // tiles in LDS: one at work, three on their way
 constexpr int kPageList = 1024;    // pages of the keys at hand
-// us, two workgroups a CU at work: a part besides its keys, a key at 128 queries, a key below
-constexpr double kPartTime = 7.0, kKeyTimeFull = 0.036, kKeyTime = 0.024;
 constexpr float kLog2e = 1.44269504088896340736f;
 // A running maximum is raised (and the sums rescaled) only once a score exceeds
 // it by this many powers of two: weights stay below 2^8, far from fp16's range.
@@ -236,7 +233,8 @@ __device__ __forceinline__ int64_t part_block(const AttnArgs& a, bool is_prefix,
 }
 
 template <int D> struct Tile {
-    static constexpr int kBytes = D == 256 ? 16384 : 8192;                     // a tile's keys (and its values) in LDS
+    static constexpr int kBytes = 16384;                                       // a tile's keys (and its values) in LDS
+    static constexpr int kStages = D == 256 ? 4 : 2;                           // tiles in LDS: one at work, the others on their way
     static constexpr int kKeys = kBytes / (2 * D), kBlocks = kKeys / 32;   // keys of a tile; blocks of 32
     static constexpr int kChunks = D / 8, kRowsPerLoad = kWave / kChunks;      // 16-byte chunks of a row; rows a load brings
     static constexpr int kWaves = 4;
@@ -246,7 +244,7 @@ template <int D> struct Tile {
 // Two workgroups fit a CU (with the sums of 256 places one, whose waves have all of a
 // SIMD's registers), so that one's start, softmax and waits run beside the other's products.
 template <int D> struct AttnLds {
-    unsigned char tiles[kStages][2][Tile<D>::kBytes];   // [stage][keys, values]
+    unsigned char tiles[Tile<D>::kStages][2][Tile<D>::kBytes];   // [stage][keys, values]
     int64_t pages[kPageList];
     int32_t bad[Tile<D>::kWaves];
 };
@@ -257,7 +255,7 @@ template <int DT, int D, int kWaves>
 __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds<D>& lds, const Scope& s, bool is_prefix,
                                             int head, int queries, int m0, int64_t k0, int64_t k1, int64_t block) {
     using T = Tile<D>;
-    constexpr int kTileBytes = T::kBytes;
+    constexpr int kTileBytes = T::kBytes, kStages = T::kStages;
     constexpr int kKeys = T::kKeys, kBlocks = T::kBlocks, kChunks = T::kChunks, kRowsPerLoad = T::kRowsPerLoad;
     constexpr int kLoads = T::kLoads, kSteps = T::kSteps, kOuts = T::kOuts;
     constexpr int kAlong = T::kWaves / kWaves < kBlocks ? T::kWaves / kWaves : kBlocks;     // waves along the keys
@@ -631,13 +629,12 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds<D>& lds, 
 template <int DT, int D>
 __global__ __launch_bounds__(Tile<D>::kWaves* kWave, D == 256 ? 1 : 2) void attend_kernel(AttnArgs a) {
     __shared__ __align__(1024) AttnLds<D> lds;
-    // Which item: prefixes' (bound by the products) spread evenly among the lanes' own (bound by
-    // memory), so that the CUs are at both at any time; heads fastest.
+    // which item: the prefixes' first, heads fastest
     const int kv_heads = a.cache.kv_heads;
-    const uint32_t prefix_items = uint32_t(a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits);
-    const int before = int(uint64_t(blockIdx.x) * prefix_items / gridDim.x);
-    const bool is_prefix = int(uint64_t(blockIdx.x + 1) * prefix_items / gridDim.x) > before;
-    int item = is_prefix ? before : int(blockIdx.x) - before;
+    const int prefix_items = a.groups * kv_heads * a.plan.prefix.tiles * a.plan.prefix.splits;
+    int item = blockIdx.x;
+    const bool is_prefix = item < prefix_items;
+    if (!is_prefix) item -= prefix_items;
     const ScopePlan& plan = is_prefix ? a.plan.prefix : a.plan.own;
     const int head = item % kv_heads;
     item /= kv_heads;
@@ -686,7 +683,7 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
 // of a part's block.
 template <int DT, int D>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
-    constexpr int kQuads = D / 4, kBatch = 4;
+    constexpr int kQuads = D / 4, kBatch = 6;
     const int per_kv = a.heads / a.cache.kv_heads;
     const int64_t t = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x;
     const int64_t span = int64_t(per_kv) * kQuads;   // threads of a (row, kv head)
@@ -698,40 +695,46 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     float top = -kInfF, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
     if (!r.lost) {
-        for (int k = 0; k < 2; ++k) {   // the group's parts, then the lane's own
-            const int parts = k ? r.own_parts : r.group_parts, which = k ? r.lane : r.group;
-            if (parts == 0) continue;
-            const int m = (k ? r.own_row : r.group_row) * per_kv + g;
-            const ScopePlan& plan = k ? a.plan.own : a.plan.prefix;
-            const int64_t first = part_block(a, !k, 0, which, kv) + m / 32;
-            const int64_t step = part_block(a, !k, 1, which, kv) + m / 32 - first;
-            const int at = (d / 8 * 2 + (d / 4 & 1)) * 32 + m % 32;   // of a block, in float4
-            for (int i0 = 0; i0 < parts; i0 += kBatch) {   // so many parts' loads in flight
-                float2 ml[kBatch];
-                float4 v[kBatch];
+        // the group's parts, then the lane's own, kBatch parts' loads in flight
+        int64_t first[2], step[2];
+        int m[2];
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int64_t block = first + min(i0 + j, parts - 1) * step;
-                    ml[j] = a.part_ml[block * 32 + m % 32];
-                    v[j] = reinterpret_cast<const float4*>(a.part_o + block * (32 * D))[at];
-                }
+        for (int k = 0; k < 2; ++k) {
+            const int which = k ? r.lane : max(r.group, 0);
+            m[k] = (k ? r.own_row : r.group_row) * per_kv + g;
+            first[k] = part_block(a, !k, 0, which, kv) + m[k] / 32;
+            step[k] = part_block(a, !k, 1, which, kv) + m[k] / 32 - first[k];
+        }
+        const int place = (d / 8 * 2 + (d / 4 & 1)) * 32;   // of a block, in float4
+        const int parts = r.group_parts + r.own_parts;
+        for (int i0 = 0; i0 < parts; i0 += kBatch) {
+            float2 ml[kBatch];
+            float4 v[kBatch];
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    if (i0 + j >= parts) break;
-                    if (__builtin_signbit(ml[j].y)) {
-                        ml[j].y = -ml[j].y;
-                        const Scope s = k ? own_scope(a, which) : prefix_scope(a, which);
-                        const float4 x = no_numbers<DT>(a, s, plan, i0 + j, row, head, d, !k);
-                        v[j].x += x.x; v[j].y += x.y; v[j].z += x.z; v[j].w += x.w;
-                    }
-                    if (ml[j].x == -kInfF && ml[j].y == 0.0f) continue;   // it saw nothing
-                    const float next = fmaxf(top, ml[j].x);
-                    const float x = rescale(top, next, a.scale2), y = rescale(ml[j].x, next, a.scale2);
-                    top = next;
-                    sum = sum * x + ml[j].y * y;
-                    o.x = o.x * x + v[j].x * y; o.y = o.y * x + v[j].y * y;
-                    o.z = o.z * x + v[j].z * y; o.w = o.w * x + v[j].w * y;
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = min(i0 + j, parts - 1), k = i >= r.group_parts;
+                const int64_t block = first[k] + (i - (k ? r.group_parts : 0)) * step[k];
+                ml[j] = a.part_ml[block * 32 + m[k] % 32];
+                v[j] = reinterpret_cast<const float4*>(a.part_o + block * (32 * D))[place + m[k] % 32];
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                if (i0 + j >= parts) break;
+                if (__builtin_signbit(ml[j].y)) {
+                    ml[j].y = -ml[j].y;
+                    const bool own = i0 + j >= r.group_parts;
+                    const Scope s = own ? own_scope(a, r.lane) : prefix_scope(a, r.group);
+                    const float4 x = no_numbers<DT>(a, s, own ? a.plan.own : a.plan.prefix,
+                                                    i0 + j - (own ? r.group_parts : 0), row, head, d, !own);
+                    v[j].x += x.x; v[j].y += x.y; v[j].z += x.z; v[j].w += x.w;
                 }
+                if (ml[j].x == -kInfF && ml[j].y == 0.0f) continue;   // it saw nothing
+                const float next = fmaxf(top, ml[j].x);
+                const float x = rescale(top, next, a.scale2), y = rescale(ml[j].x, next, a.scale2);
+                top = next;
+                sum = sum * x + ml[j].y * y;
+                o.x = o.x * x + v[j].x * y; o.y = o.y * x + v[j].y * y;
+                o.z = o.z * x + v[j].z * y; o.w = o.w * x + v[j].w * y;
             }
         }
     } else {
@@ -763,27 +766,22 @@ AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int gr
     p.prefix = scope_plan(int64_t(std::max(max_group_rows, 1)) * per_kv);
     const int64_t own_items = int64_t(lanes) * kv_heads * p.own.tiles;
     const int64_t prefix_items = int64_t(groups) * kv_heads * p.prefix.tiles;
-    // Of some lengths of time, the one for which the work is done first if every workgroup
-    // gets as many keys as fit it.
-    const double slots = double(device_cus()) * (head_dim == 256 ? 1 : 2);
-    auto key_time = [&](const ScopePlan& scope) { return scope.waves == 4 ? kKeyTimeFull : kKeyTime; };
-    auto splits = [&](const ScopePlan& scope, int64_t keys, double time) {
-        return int64_t(std::clamp(__builtin_ceil(double(keys) * key_time(scope) / (time - kPartTime)), 1.0, 128.0));
-    };
-    auto part_time = [&](const ScopePlan& scope, int64_t keys, int64_t n) {
-        return kPartTime + key_time(scope) * double((keys + n - 1) / n);
-    };
-    double least = 0.0;
-    int64_t own_splits = 1, prefix_splits = 1;
-    for (double time = kPartTime + 2.0; time < 2e4; time *= 1.12) {
-        const int64_t n = splits(p.own, max_own, time), m = splits(p.prefix, max_prefix, time);
-        const double own = part_time(p.own, max_own, n), prefix = groups ? part_time(p.prefix, max_prefix, m) : 0.0;
-        const double longest = std::max(own, prefix), items = double(own_items * n) + (groups ? double(prefix_items * m) : 0.0);
-        const double all = (double(own_items * n) * own + (groups ? double(prefix_items * m) * prefix : 0.0)) / slots;
-        const double done = items <= slots ? longest : all + 0.5 * longest;
-        if (least == 0.0 || done < least) { least = done; own_splits = n; prefix_splits = m; }
-        if (n == 1 && m == 1) break;
+    // The prefixes' parts are bound by the products, the lanes' own by memory: where both are
+    // work, a CU has one of each, the prefixes' (launched first) one a CU, and the own ones what
+    // is left, in parts of at most 704 keys that fill the gaps.  64 x 1 rows over 32,768 shared
+    // and 2,048 own keys, 8 kv heads: 144 us so, 155 with own parts of 2,112 keys, 172 with
+    // two prefix parts a CU; the prefix alone 99 us with two parts a CU.
+    const int64_t slots = int64_t(device_cus()) * (head_dim == 256 ? 1 : 2), least = 2 * tile;
+    const int64_t own_work = own_items * max_own, prefix_work = prefix_items * max_prefix;
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    int64_t prefix_splits = 0;
+    if (groups) {
+        const int64_t share = own_work * 8 < prefix_work ? slots : std::max<int64_t>(slots / 2, 1);
+        prefix_splits = std::clamp<int64_t>(std::min(share / prefix_items, up(max_prefix, least)), 1, 128);
     }
+    const int64_t rest = std::max<int64_t>(slots - prefix_items * prefix_splits, 1);
+    const int64_t own_splits =
+        std::clamp<int64_t>(std::min(std::max(rest / own_items, up(max_own, 704)), up(max_own, least)), 1, 128);
     auto cut = [&](ScopePlan& scope, int64_t keys, int64_t n) {   // into chunks alike
         scope.splits = int(n);
         const int64_t each = (std::max<int64_t>(keys, 1) + scope.splits - 1) / scope.splits;
