@@ -108,6 +108,28 @@ __global__ __launch_bounds__(256) void truncate_kernel(vi_page_map m, const int3
     if (threadIdx.x == 0) m.lengths[lane] = length;
 }
 
+// Exclusive prefixes of two values of a thread over the workgroup, and their sums.
+__device__ __forceinline__ void block_exclusive_scan_pair(uint32_t& x, uint32_t& y, uint32_t* tmp, uint32_t* sum_x,
+                                                          uint32_t* sum_y) {
+    constexpr int kWaves = kPlan / kWave;
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    const uint32_t ix = wave_incl_scan_u32(x), iy = wave_incl_scan_u32(y);
+    if (lane == kWave - 1) { tmp[wave] = ix; tmp[kWaves + 1 + wave] = iy; }
+    __syncthreads();
+    if (wave < 2) {   // the wave totals of x in wave 0, of y in wave 1
+        uint32_t* const t = tmp + wave * (kWaves + 1);
+        const uint32_t v = lane < kWaves ? t[lane] : 0u, i = wave_incl_scan_u32(v);
+        if (lane < kWaves) t[lane] = i - v;
+        if (lane == kWaves - 1) t[kWaves] = i;
+    }
+    __syncthreads();
+    x = tmp[wave] + ix - x;
+    y = tmp[kWaves + 1 + wave] + iy - y;
+    *sum_x = tmp[kWaves];
+    *sum_y = tmp[2 * kWaves + 1];
+    __syncthreads();
+}
+
 // ---- extend -----------------------------------------------------------------------
 struct ExtendWs {
     uint32_t* pairs;      // planned copies
@@ -125,8 +147,19 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
     __shared__ uint32_t sharers[kShareSlots];
     __shared__ uint32_t lasts[kShareSlots];
     __shared__ uint32_t base[kListMax + 1];
-    __shared__ uint32_t tmp[kPlan / kWave + 1];
+    __shared__ uint32_t tmp[2 * (kPlan / kWave + 1)];
     const int tid = threadIdx.x;
+    // which of the thread's four pages of a chunk are free
+    auto free_of = [&](int p0) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = p0 + tid * 4 + j;
+            if (p < m.pages && m.refs[p] == 0) bits |= 1u << j;
+        }
+        return bits;
+    };
+    const uint32_t first_free = free_of(0);   // (requested beside the list)
     int slots = 64;
     while (slots < 2 * count) slots <<= 1;
     const int shift = 32 - __builtin_ctz(unsigned(slots));
@@ -180,19 +213,14 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
         copies += copied[k];
     }
     uint32_t total, pairs;
-    uint32_t at = block_exclusive_scan_u32<kPlan>(mine, tmp, &total);
-    uint32_t pair = block_exclusive_scan_u32<kPlan>(copies, tmp, &pairs);
-    // enough free pages?  (the counts are read again below, from L2)
-    uint32_t free_pages = 0;
-    for (int p0 = 0; p0 < m.pages && free_pages < total; p0 += kPlan * 4) {
-        uint32_t mine_free = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = p0 + tid * 4 + j;
-            mine_free += p < m.pages && m.refs[p] == 0;
-        }
+    uint32_t at = mine, pair = copies;
+    block_exclusive_scan_pair(at, pair, tmp, &total, &pairs);
+    // enough free pages?  (the first chunk's stay at hand, later ones are read again below)
+    uint32_t free_pages, first_rank = block_exclusive_scan_u32<kPlan>(uint32_t(__builtin_popcount(first_free)), tmp, &free_pages);
+    const uint32_t first_sum = free_pages;
+    for (int p0 = kPlan * 4; p0 < m.pages && free_pages < total; p0 += kPlan * 4) {
         uint32_t sum;
-        block_exclusive_scan_u32<kPlan>(mine_free, tmp, &sum);
+        block_exclusive_scan_u32<kPlan>(uint32_t(__builtin_popcount(free_of(p0))), tmp, &sum);
         free_pages += sum;
     }
     if (refused || free_pages < total) {
@@ -235,22 +263,10 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
         pair += copied[k];
     }
     __syncthreads();
-    uint32_t done = 0;
-    for (int p0 = 0; p0 < m.pages && done < total; p0 += kPlan * 4) {
-        uint32_t mine_free = 0;
-        bool is_free[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = p0 + tid * 4 + j;
-            is_free[j] = p < m.pages && m.refs[p] == 0;
-            mine_free += is_free[j];
-        }
-        uint32_t sum, rank = done + block_exclusive_scan_u32<kPlan>(mine_free, tmp, &sum);
-        done += sum;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!is_free[j] || rank >= total) continue;
-            const int p = p0 + tid * 4 + j;
+    uint32_t done = first_sum;
+    auto hand_out = [&](int p0, uint32_t bits, uint32_t rank) {
+        for (; bits && rank < total; bits &= bits - 1u, ++rank) {
+            const int p = p0 + tid * 4 + __builtin_ctz(bits);
             int lo = 0, hi = count - 1;   // the last lane whose first rank is not above this one
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -260,8 +276,15 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
             m.tables[int64_t(who[lo]) * m.table_stride + held_l - copy + e] = p;
             m.refs[p] = 1;
             if (copy && e == 0) w.targets[order[lo]] = p;
-            ++rank;
         }
+    };
+    hand_out(0, first_free, first_rank);
+    for (int p0 = kPlan * 4; p0 < m.pages && done < total; p0 += kPlan * 4) {
+        const uint32_t bits = free_of(p0);
+        uint32_t sum;
+        const uint32_t rank = done + block_exclusive_scan_u32<kPlan>(uint32_t(__builtin_popcount(bits)), tmp, &sum);
+        done += sum;
+        hand_out(p0, bits, rank);
     }
 #pragma unroll
     for (int k = 0; k < kListPer; ++k) {
@@ -356,35 +379,47 @@ constexpr int kKeepBatch = 4;   // vectors a thread holds between the reads and 
 // path, so batches in path order never overwrite a row that is still to be
 // read; within a batch every read comes before every write.
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
-    const int i = blockIdx.x / a.pool.planes, plane = blockIdx.x % a.pool.planes, tid = threadIdx.x;
+    const int i = int(blockIdx.x / uint32_t(a.pool.planes)), plane = int(blockIdx.x % uint32_t(a.pool.planes)), tid = threadIdx.x;
     const int lane = a.lane_ids[i];
     if (uint32_t(lane) >= uint32_t(a.m.lanes)) return;
     const int32_t* const path = a.paths + int64_t(i) * a.path_stride;
     const int32_t* const table = a.m.tables + int64_t(lane) * a.m.table_stride;
-    const int context = a.context[i], n = min(a.kept[i], a.path_stride), per_row = a.kv_heads * a.vecs;
+    const int context = a.context[i], n = min(a.kept[i], a.path_stride);
+    const uint32_t per_row = uint32_t(a.kv_heads) * uint32_t(a.vecs);
     if (context < 0) return;
     unsigned char* const base = static_cast<unsigned char*>(a.pool.base) + int64_t(plane) * a.pool.plane_stride;
-    auto place = [&](int64_t index, int head, int vec) -> uint4* {
-        const int64_t e = index / a.m.page_size;
-        if (index < 0 || e >= a.m.table_width) return nullptr;
+    const int shift = __builtin_ctz(unsigned(a.m.page_size));
+    auto place = [&](int64_t index, uint32_t head, uint32_t vec) -> uint4* {
+        const int64_t e = index >> shift;
+        if (e >= a.m.table_width) return nullptr;
         const int page = table[e];
         if (uint32_t(page) >= uint32_t(a.m.pages)) return nullptr;
         return reinterpret_cast<uint4*>(base + int64_t(page) * a.pool.page_bytes) +
-               (int64_t(head) * a.m.page_size + index % a.m.page_size) * a.vecs + vec;
+               ((head << shift) + (uint32_t(index) & uint32_t(a.m.page_size - 1))) * uint32_t(a.vecs) + vec;
     };
-    int j0 = 0;   // rows that stay in place need nothing
-    while (j0 < n && path[j0] == j0) ++j0;
-    const int64_t items = int64_t(n - j0) * per_row;
-    for (int64_t b = 0; b < items; b += kKeepThreads * kKeepBatch) {
+    // rows that stay in place need nothing: the first that moves, found by all threads at once
+    __shared__ int first_move;
+    if (tid == 0) first_move = n;
+    __syncthreads();
+    for (int j = tid; j < n; j += kKeepThreads)
+        if (path[j] != j) {
+            atomicMin(&first_move, j);
+            break;
+        }
+    __syncthreads();
+    const int j0 = first_move;
+    if (j0 >= n) return;
+    const uint32_t items = uint32_t(n - j0) * per_row;
+    for (uint32_t b = 0; b < items; b += kKeepThreads * kKeepBatch) {
         uint4 v[kKeepBatch];
         uint4* to[kKeepBatch];
 #pragma unroll
         for (int k = 0; k < kKeepBatch; ++k) {
-            const int64_t it = b + k * kKeepThreads + tid;
+            const uint32_t it = b + k * kKeepThreads + tid;
             to[k] = nullptr;
             if (it >= items) continue;
-            const int j = j0 + int(it / per_row), head = int(it % per_row) / a.vecs, vec = int(it % a.vecs);
-            const int from = path[j];
+            const uint32_t row = it / per_row, in = it - row * per_row, head = in / uint32_t(a.vecs), vec = in - head * uint32_t(a.vecs);
+            const int j = j0 + int(row), from = path[j];
             if (from <= j || from >= 65536 || (j > 0 && path[j - 1] >= from)) continue;
             const uint4* const src = place(int64_t(context) + from, head, vec);
             to[k] = place(int64_t(context) + j, head, vec);
@@ -451,6 +486,10 @@ vi_status launch_pages_compact(const vi_page_map& m, const vi_page_pool& pool, v
 vi_status launch_keep_rows(const vi_page_map& m, const vi_page_pool& pool, int kv_heads, const int32_t* lane_ids,
                            const int32_t* context, const int32_t* paths, int path_stride, const int32_t* kept,
                            int count, hipStream_t stream) {
+    // (the kernel's places in a lane's path and in a page are 32-bit)
+    if (int64_t(path_stride) * (pool.page_bytes / 16 / m.page_size) > 0x7fffffff || pool.page_bytes > 0x7fffffff ||
+        int64_t(count) * pool.planes > 0x7fffffff)
+        return VI_ERR_UNSUPPORTED;
     KeepArgs a{m, pool, kv_heads, int(pool.page_bytes / (int64_t(kv_heads) * m.page_size * 16)), path_stride,
                lane_ids, context, paths, kept};
     hipLaunchKernelGGL(keep_kernel, dim3(unsigned(count) * pool.planes), dim3(kKeepThreads), 0, stream, a);
