@@ -232,6 +232,23 @@ def test_refused_on_the_device(dev, rng, calls):
     same(m, d, "after")
 
 
+def test_lengths_at_the_end_of_32_bits(dev, rng):
+    """A length whose number of pages needs the carry out of 31 bits is refused like any that is too long; a lane
+    that claims so many tokens is cut back to the pages that its table has."""
+    m = Model(3, 9, 60, 16, 1, 1, 8, rng)
+    d = Device(m, dev)
+    for kind, *args in [("extend", [0, 1], [40, 20]), ("extend", [0], [2**31 - 1]), ("extend", [1, 2], [2**31 - 5, 3])]:
+        getattr(m, kind)(*args)
+        getattr(d, kind)(*args)
+        same(m, d, (kind, args))
+    assert m.status[0] == FLAG_ERROR
+    m.lengths[0] = 2**31 - 1
+    d.lengths[0] = 2**31 - 1
+    m.truncate([0], [17])
+    d.truncate([0], [17])
+    same(m, d, "truncate")
+
+
 def test_copy_pages(dev, rng):
     import voidinfer_amd as vi
     pool = torch.from_numpy(rng.standard_normal((3, 2, 50, 2, 16, 8)).astype(np.float32)).to(dev).to(torch.bfloat16)

@@ -1,11 +1,20 @@
 // append.hip — norms of queries and keys per head, their rotation, and the rows'
 // keys and values written to the lanes' pages, in one pass (vi_norm_rotate_append).
 //
+// y = x / sqrt(mean(x^2) + eps) * w, then the first places turned by the row's
+// angles, all in fp32 and rounded once to the cache's type.
+//
 // A head vector is read once and written once: the kernel is bound by those
 // bytes.  Each thread holds two 16-byte chunks of one head, the two whose elements
 // turn together (i and i + rotary/2) where the rotation is by halves, so the
 // rotation needs no exchange; the mean square is summed in fp32 over the threads
 // of a head, a power of two of them, by lane exchanges.
+//
+// 16,384 rows of 32 + 2 x 8 heads of 128 bf16 places (403 MB both ways): 102 to 106
+// us, 3.9 TB/s against 4.8 of a plain copy; 8 rows 5.1 us and 136 rows 5.8 us, the
+// look-ups of lane, page and angle one behind the other.  One head a thread: with
+// two and four, whose look-ups are shared, the long case takes 112 to 114 us
+// (fewer loads in flight a wave) and 8 rows 6.4 to 8.4.
 #include "cache_rows.h"
 
 namespace vi {

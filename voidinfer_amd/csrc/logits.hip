@@ -1,13 +1,26 @@
 // logits.hip — rows of logits rewritten by penalties, biases and grammar masks
 // before a decision is taken over them (vi_process_logits).
 //
+// x' = pen(x, occurrences) + bias in fp32, -Inf where the grammar forbids, rounded
+// once to the logits' type; a logit that no rule touches keeps its bits.
+//
 // One workgroup per (row, slice of 8,192 tokens).  A token's penalty needs its
 // number of occurrences, a bias the last entry that names it: both are rare in a
 // slice, so each thread requests its logits first (they stay in registers),
 // then the workgroup goes over the lane's lists and notes what falls into the
 // slice in LDS: a bitmap of touched tokens and a counter per token, then, in the
-// same array, the biases' places in their list.  Vectors whose part of a bitmap
-// is zero go through unread and unrounded.
+// same array, the biases' places in their list.  A vector that the masks forbid
+// whole is not read.
+//
+// Bound: the row read and written once, and every slice's reading of the lists (a
+// history of 4,096 tokens is as many bytes as a bf16 slice, from the L2).  136
+// rows of 248,320 bf16, half of them masked, histories of 4,096: 37.8 us, 3.6 TB/s
+// of rows and lists against 4.8 of a plain copy; one row of 151,936 fp32 6.4 us
+// and 64 of 65,537 fp16 10.5 us, both the wait for parameters, lists and logits
+// one behind the other.  512 threads and 8,192 tokens (36 KB of LDS: four
+// workgroups, all waves of a CU): with 1,024 threads and 16,384 tokens the 136
+// rows take 58.9 us, with 256 and 4,096 42.0, 512 and 16,384 81.6 (two workgroups a
+// CU), 256 and 8,192 67.
 #include <algorithm>
 
 #include "penalty_state.h"
@@ -262,7 +275,7 @@ vi_status launch_rules(const void* logits, int dtype, int rows, int vocabulary, 
                        hipStream_t stream) {
     RuleArgs a{};
     a.logits = logits; a.out = out; a.stride = stride; a.out_stride = out_stride;
-    a.rows = rows; a.vocabulary = vocabulary; a.slices = (vocabulary + kRuleSlice - 1) / kRuleSlice;
+    a.rows = rows; a.vocabulary = vocabulary; a.slices = (vocabulary - 1) / kRuleSlice + 1;
     a.r = rules; a.row_flags = row_flags;
     if (rules.states) a.layout = penalty_layout(vocabulary, rules.slots);
     const bool lists = rules.bias_ids || (rules.params && (rules.histories || rules.states || rules.extra));
