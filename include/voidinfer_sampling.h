@@ -513,7 +513,7 @@ vi_status vi_norm_rotate_append(const vi_kv_cache* cache, const vi_lane_rows* la
  * (tokens of a lane past its group's prefix, its rows included) and max_prefix
  * choose the split of the work and size the workspace; lengths past max_own or
  * max_prefix are still read, rows past max_rows or max_group_rows get NaN.
- * head_dim: 64, 128 or 256; bf16 or fp16. */
+ * head_dim: 64, 128 or 256; bf16 or fp16; token_stride below 2^31 / page_size. */
 size_t vi_prefix_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int lanes, int groups,
                                            int max_rows, int max_group_rows, int64_t max_own, int64_t max_prefix);
 vi_status vi_prefix_attention(const vi_kv_cache* cache, const vi_lane_rows* lanes, int heads,

@@ -96,7 +96,8 @@ def test_append_refuses_caches(lib, want, kw):
                                      128, 0, 0) == want
 
 
-@pytest.mark.parametrize("want,kw", CACHE_FAULTS + [(UNSUPPORTED, dict(head_dim=96))])
+@pytest.mark.parametrize("want,kw", CACHE_FAULTS + [(UNSUPPORTED, dict(head_dim=96)),
+                                                    (UNSUPPORTED, dict(token_stride=1 << 27))])
 def test_attention_refuses_caches(lib, want, kw):
     assert lib.vi_prefix_attention(cache(**kw), lane_rows(), 8, heads(), 0.1, 0, 0, 0, 4, 0, 10, 0, 0, P, 1024, 128, 0,
                                    P, 1 << 30, 0) == want

@@ -15,6 +15,26 @@
 // ahead; 16-byte chunks of a row are permuted by the row's number, so that the
 // 16 rows that a fragment read touches at once, and the 4 rows x 64 bytes of a
 // transposing read, fall into different banks.
+//
+// Rounding: queries, keys and values are 16 bits as given, scores, maxima, sums and
+// outputs fp32, the output rounded once.  The weights are rounded to the cache's type
+// for the second product (the matrix instructions take 16 bits on both sides; an
+// fp32 product would be sixteen times slower); they are in 0 .. 2^8 with a relative error of
+// 2^-9 (bf16) or 2^-11 each, while their sum is taken before the rounding.
+//
+// Bound and measured.  64 x 1 rows of 64 heads (8 of keys and values, 128 places, bf16)
+// over 32,768 shared and up to 2,048 own keys: 146 us for 72 GFLOP and 0.55 GB, the prefix
+// alone 99 us (0.7 PFLOP/s; a library product of 8,192^3 reaches 1.2), the join 9.
+// The matrix instructions of a wave's 32 queries need as much of LDS (each fragment
+// is read for 32 queries) as of the SIMD, and the softmax about as much of the
+// vector units; two workgroups a CU overlap these in part.  8 x 17 rows of 32 heads
+// over 4,096 shared and up to 1,500 own keys: 30 us, and 10 for the join (23 MB of parts).
+// 4 x 1 rows of 16 heads of 64 places over 512 and 100: 9 + 4 us, of which 5 the look-ups
+// before a part's first load (offsets, lengths, group, table, page).
+// Not taken: eight waves over 256 queries in step, one of a SIMD at the products while
+// the other is at its weights (180 to 200 us for the first case: no room for own
+// parts beside a prefix part); tiles of 32 keys four deep (160 to 214 us); prefix
+// and own parts launched alternately (the prefix alone 143 us).
 #include <algorithm>
 
 #include "cache_rows.h"
@@ -40,7 +60,7 @@ struct RowInfo {
     int32_t lane, group;        // group: -1 without
     int32_t own_row, group_row; // the row's place in the two scopes
     int32_t own_parts, group_parts;
-    int32_t lost;               // outside the caller's bounds
+    int32_t lost;               // set by the join: outside the caller's bounds
     int32_t reserved;
 };
 
@@ -184,7 +204,8 @@ __device__ __forceinline__ Scope own_scope(const AttnArgs& a, int lane) {
 }
 __device__ __forceinline__ Scope prefix_scope(const AttnArgs& a, int g) {
     Scope s;
-    const int first = a.group_offsets[g], last = a.group_offsets[g + 1];
+    const int first = min(max(a.group_offsets[g], 0), a.lanes.lanes - 1);
+    const int last = min(a.group_offsets[g + 1], a.lanes.lanes);
     s.row0 = a.lanes.row_offsets[first];
     s.rows = last > first ? a.lanes.row_offsets[last] - s.row0 : 0;
     s.table = first;
@@ -216,11 +237,11 @@ __device__ __forceinline__ void row_info(const AttnArgs& a, const Scope& own, in
             group_row0 = p.row0;
         }
     }
-    for (int i = threadIdx.x; i < own.rows; i += blockDim.x) {
+    for (int i = threadIdx.x; i < min(own.rows, a.lanes.rows); i += blockDim.x) {
         r.own_row = i;
         r.group_row = own.row0 + i - group_row0;
-        r.lost = i >= a.max_rows || (r.group >= 0 && r.group_row >= a.max_group_rows);
-        if (own.row0 + i < a.lanes.rows) a.info[own.row0 + i] = r;
+        r.lost = 0;   // (the join finds the rows outside the caller's bounds by these)
+        if (uint32_t(own.row0 + i) < uint32_t(a.lanes.rows)) a.info[own.row0 + i] = r;
     }
 }
 
@@ -269,7 +290,7 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds<D>& lds, 
     const int qi = wave % kWaves, ki = wave / kWaves;
     const int m = m0 + qi * 32 + col;
     const bool active = m0 + qi * 32 < queries && ki < kAlong;
-    const bool live = active && m < queries;
+    const bool live = active && m < queries && uint32_t(s.row0 + m / per_kv) < uint32_t(a.lanes.rows);
     const int own_row = live ? m / per_kv : 0, row = s.row0 + own_row;
     const int qhead = head * per_kv + (live ? m % per_kv : 0);
     s16x8_t qf[kSteps];
@@ -691,7 +712,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
     const int kv = int(t / span % a.cache.kv_heads), in = int(t % span);
     const int g = in % per_kv, d = in / per_kv * 4, head = kv * per_kv + g;
-    const RowInfo r = a.info[row];
+    RowInfo r = a.info[row];
+    // (a row that no lane holds, of offsets that do not begin at 0 or fall, has whatever lay there)
+    r.own_parts = min(r.own_parts, a.plan.own.splits);
+    r.group_parts = min(r.group_parts, r.group < 0 ? 0 : a.plan.prefix.splits);
+    if (uint32_t(r.lane) >= uint32_t(a.lanes.lanes) || r.group >= a.groups || uint32_t(r.own_row) >= uint32_t(a.max_rows) ||
+        (r.group >= 0 && uint32_t(r.group_row) >= uint32_t(a.max_group_rows)))
+        r.lost = 1;
     float top = -kInfF, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
     if (!r.lost) {

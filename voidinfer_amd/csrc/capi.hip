@@ -407,7 +407,10 @@ vi_status vi_prefix_attention(const vi_kv_cache* cache, const vi_lane_rows* lane
         groups < 0 || groups > lanes->lanes || (groups && (!group_offsets || !prefix_lens)) || max_rows <= 0 ||
         max_own < 0 || max_prefix < 0 || (groups && max_group_rows <= 0) || !(scale == scale))
         return VI_ERR_INVALID;
-    if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256) return VI_ERR_UNSUPPORTED;
+    // (the kernel steps through a page's tokens in 32 bits)
+    if ((cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256) ||
+        cache->token_stride > (int64_t(1) << 31) / cache->page_size - 1)
+        return VI_ERR_UNSUPPORTED;
     return launch_attention(*cache, *lanes, heads, *queries, scale, groups, group_offsets, prefix_lens, max_rows,
                             max_group_rows, max_own, max_prefix, tree, out, out_row_stride, out_head_stride, lse,
                             workspace, workspace_bytes, as_stream(stream));
