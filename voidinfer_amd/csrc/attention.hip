@@ -24,11 +24,11 @@
 //
 // Bound and measured.  64 x 1 rows of 64 heads (8 of keys and values, 128 places, bf16)
 // over 32,768 shared and up to 2,048 own keys: 146 us for 72 GFLOP and 0.55 GB, the prefix
-// alone 99 us (0.7 PFLOP/s; a library product of 8,192^3 reaches 1.2), the join 9.
+// alone 99 us (0.7 PFLOP/s; a library product of 8,192^3 reaches 1.2), the join 9 to 11.
 // The matrix instructions of a wave's 32 queries need as much of LDS (each fragment
 // is read for 32 queries) as of the SIMD, and the softmax about as much of the
 // vector units; two workgroups a CU overlap these in part.  8 x 17 rows of 32 heads
-// over 4,096 shared and up to 1,500 own keys: 30 us, and 10 for the join (23 MB of parts).
+// over 4,096 shared and up to 1,500 own keys: 29 us, and 8 for the join (23 MB of parts).
 // 4 x 1 rows of 16 heads of 64 places over 512 and 100: 9 + 4 us, of which 5 the look-ups
 // before a part's first load (offsets, lengths, group, table, page).
 // Not taken: eight waves over 256 queries in step, one of a SIMD at the products while
@@ -42,7 +42,7 @@
 namespace vi {
 namespace {
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256;   // 32 queries x 8 times 4 places
 constexpr int kPageList = 1024;    // pages of the keys at hand
 constexpr float kLog2e = 1.44269504088896340736f;
 // A running maximum is raised (and the sums rescaled) only once a score exceeds
@@ -699,19 +699,20 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
     return make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// The parts of every (row, head) joined.  Thread by thread the query heads of one kv
-// head and row, then the places, four each: neighbours read neighbouring queries
-// of a part's block.
+// The parts of every (row, head) joined.  A workgroup takes 32 queries of a kv head
+// (rows x query heads) and 32 places, four a thread: its reads of a part are whole
+// lines where the queries lie in one block of the part.  (8 x 17 rows of 32 heads: 8.2
+// us, 10.4 with a row's places and heads by neighbouring threads, 64 bytes together.
+// Six parts' loads in flight: with 3 or 12 the same, or up to 2 us more.)
 template <int DT, int D>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
-    constexpr int kQuads = D / 4, kBatch = 6;
+    constexpr int kBatch = 6;
     const int per_kv = a.heads / a.cache.kv_heads;
-    const int64_t t = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x;
-    const int64_t span = int64_t(per_kv) * kQuads;   // threads of a (row, kv head)
-    const int row = int(t / (span * a.cache.kv_heads));
+    const int d = int(blockIdx.x % (D / 32)) * 32 + int(threadIdx.x / 32) * 4;
+    const int kv = int(blockIdx.x / (D / 32) % unsigned(a.cache.kv_heads));
+    const int64_t query = int64_t(blockIdx.x / (D / 32) / unsigned(a.cache.kv_heads)) * 32 + threadIdx.x % 32;
+    const int row = int(query / per_kv), g = int(query % per_kv), head = kv * per_kv + g;
     if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
-    const int kv = int(t / span % a.cache.kv_heads), in = int(t % span);
-    const int g = in % per_kv, d = in / per_kv * 4, head = kv * per_kv + g;
     RowInfo r = a.info[row];
     // (a row that no lane holds, of offsets that do not begin at 0 or fall, has whatever lay there)
     r.own_parts = min(r.own_parts, a.plan.own.splits);
@@ -824,11 +825,14 @@ size_t attention_blocks(const AttnPlan& p, int kv_heads, int lanes, int groups) 
                                size_t(p.prefix.splits) * groups * p.prefix.tiles * p.prefix.waves);
 }
 
+int64_t join_blocks(const AttnArgs& a) {
+    const int64_t queries = int64_t(a.lanes.rows) * (a.heads / a.cache.kv_heads);
+    return (queries + 31) / 32 * a.cache.kv_heads * (a.cache.head_dim / 32);
+}
+
 template <int DT, int D> void launch_dim(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(Tile<D>::kWaves * kWave), 0, stream, a);
-    const int64_t threads = int64_t(a.lanes.rows) * a.heads * (D / 4);
-    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned((threads + kJoinThreads - 1) / kJoinThreads)),
-                       dim3(kJoinThreads), 0, stream, a);
+    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned(join_blocks(a))), dim3(kJoinThreads), 0, stream, a);
 }
 template <int DT> void launch_type(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     switch (a.cache.head_dim) {
@@ -871,8 +875,7 @@ vi_status launch_attention(const vi_kv_cache& cache, const vi_lane_rows& lanes, 
     if (!c.ok) return VI_ERR_WORKSPACE;
     const int64_t blocks = (int64_t(groups) * a.plan.prefix.tiles * a.plan.prefix.splits +
                             int64_t(lanes.lanes) * a.plan.own.tiles * a.plan.own.splits) * cache.kv_heads;
-    if (blocks > 0x7fffffff || int64_t(lanes.rows) * heads * (cache.head_dim / 4) > int64_t(0x7fffffff) * kJoinThreads)
-        return VI_ERR_UNSUPPORTED;
+    if (blocks > 0x7fffffff || join_blocks(a) > 0x7fffffff) return VI_ERR_UNSUPPORTED;
     if (cache.dtype == VI_BF16) launch_type<VI_BF16>(a, unsigned(blocks), stream);
     else launch_type<VI_F16>(a, unsigned(blocks), stream);
     return launch_status();
