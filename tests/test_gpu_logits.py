@@ -259,3 +259,9 @@ def test_refusals_on_the_device_side(dev):
                dict(histories=i32, offsets=off[:2], params=vi.params_array(2))):
         with pytest.raises(ValueError):
             vi.process_logits(x, **kw)
+
+
+def test_masks_in_host_memory_are_refused(dev):
+    x = torch.zeros(2, 64, device=dev)
+    with pytest.raises(ValueError):
+        vi.process_logits(x, masks=torch.zeros(1, 2, dtype=torch.int32), mask_index=torch.zeros(2, dtype=torch.int32, device=dev))

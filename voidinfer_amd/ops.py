@@ -459,8 +459,8 @@ def process_logits(logits: torch.Tensor, params: np.ndarray | torch.Tensor | Non
         bo = _int_list(bias_offsets, torch.int64, "bias_offsets")
     if mask_index is not None:
         if masks is None or masks.dtype != torch.int32 or masks.dim() != 2 or masks.stride(1) != 1 or \
-                masks.shape[1] * 32 < vocab:
-            raise ValueError("masks must be int32 [n, ceil(vocabulary / 32)] with contiguous rows")
+                masks.shape[1] * 32 < vocab or not masks.is_cuda:
+            raise ValueError("masks must be int32 [n, ceil(vocabulary / 32)] device memory with contiguous rows")
         mi = _int_list(mask_index, torch.int32, "mask_index", rows)
         m, n_masks, stride_m = masks.data_ptr(), masks.shape[0], max(masks.stride(0), masks.shape[1])
     elif masks is not None:
