@@ -211,3 +211,14 @@ def test_host_tensors_and_shapes_are_refused():
         vi.pages_fork(i, t, i[:1], i, i, 16)
     with pytest.raises(ValueError):
         vi.pages_copy(pages, i, i)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("device_list", (1, torch.int32, "x", None)), ("device_list", (torch.zeros(2), 3, "x", None)),
+    ("device_list", (torch.zeros(2), torch.int32, "x")), ("kv_cache", (None, None)), ("lane_rows", (1, 2, 3, 4)),
+    ("head_rows", (None, 1, 1, 1, None, "q")), ("rotation", (1, 2, None, 1, False)), ("page_map", (None,) * 5),
+    ("table_map", (None, 1, 1)), ("page_pool", (None, 1)), ("page_pool", (None,))])
+def test_binding_refuses_what_is_no_tensor(name, args):
+    from voidinfer_amd import _binding
+    with pytest.raises((TypeError, ValueError)):
+        getattr(_binding, name)(*args)

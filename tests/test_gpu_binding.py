@@ -1,0 +1,46 @@
+"""Host structs packed from tensors: the bytes that the header's layout asks for."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_structs_of_tensors(dev):
+    from voidinfer_amd import _abi, _binding as b
+    pool = torch.zeros(3, 2, 7, 4, 16, 64, dtype=torch.float16, device=dev)
+    k, v = pool[1, 0], pool[1, 1]
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
+    assert b.kv_cache(k, v) == _abi.KV_CACHE.pack(k.data_ptr(), v.data_ptr(), 4096, 1024, 64, _abi.F16, 7, 16, 4, 64, 0)
+    tables, offsets, context = torch.zeros(5, 12, dtype=torch.int32, device=dev)[:, :9], i32(6), i32(5)
+    assert b.lane_rows(tables, offsets, context, 11) == _abi.LANE_ROWS.pack(
+        offsets.data_ptr(), context.data_ptr(), tables.data_ptr(), 12, 9, 5, 11, 0)
+    x = torch.zeros(11, 10, 64, dtype=torch.float16, device=dev)[:, 2:6]
+    assert b.head_rows(x, 11, 4, 64, k, "x") == _abi.HEAD_ROWS.pack(x.data_ptr(), 640, 64)
+    cos, sin, at = torch.zeros(50, 16, device=dev), torch.zeros(50, 16, device=dev), i32(11)
+    assert b.rotation(cos, sin, at, 11, True) == _abi.ROTATION.pack(cos.data_ptr(), sin.data_ptr(), at.data_ptr(), 50, 32, 1, 0)
+    assert b.rotation(None, None, None, 11, False) == _abi.ROTATION.pack(0, 0, 0, 0, 0, 0, 0)
+    refs, lengths, status = i32(7), i32(5), i32(3)
+    assert b.page_map(refs, tables, lengths, 16, status) == _abi.PAGE_MAP.pack(
+        refs.data_ptr(), tables.data_ptr(), lengths.data_ptr(), status.data_ptr(), 12, 7, 16, 5, 9)
+    assert b.page_map(refs, tables, None, 16, None) == _abi.PAGE_MAP.pack(refs.data_ptr(), tables.data_ptr(), 0, 0, 12, 7, 16, 5, 9)
+    assert b.table_map(tables, 7, 16) == _abi.PAGE_MAP.pack(0, tables.data_ptr(), 0, 0, 12, 7, 16, 5, 9)
+    assert b.page_pool(pool, 7) == _abi.PAGE_POOL.pack(pool.data_ptr(), 7 * 8192, 8192, 6, 0)
+    assert b.device_list(at, torch.int32, "at", 11) == at.data_ptr()
+
+
+@pytest.mark.parametrize("call", [
+    lambda b, d: b.kv_cache(d[0], d[0][:, :1]), lambda b, d: b.kv_cache(d[0].float(), d[0].float()),
+    lambda b, d: b.kv_cache(d[0].transpose(2, 3), d[0].transpose(2, 3)), lambda b, d: b.kv_cache(d[0][0], d[0][0]),
+    lambda b, d: b.head_rows(d[1], 4, 4, 64, d[0], "x"), lambda b, d: b.head_rows(d[1].float(), 3, 4, 64, d[0], "x"),
+    lambda b, d: b.head_rows(d[1].transpose(1, 2), 3, 64, 4, d[0], "x"),
+    lambda b, d: b.device_list(d[2], torch.int64, "x", None), lambda b, d: b.device_list(d[2], torch.int32, "x", 7),
+    lambda b, d: b.device_list(d[2][::2], torch.int32, "x", None),
+    lambda b, d: b.lane_rows(d[2], d[2], d[2], 1), lambda b, d: b.table_map(d[3].T, 1, 16),
+    lambda b, d: b.page_pool(d[0], 8), lambda b, d: b.page_pool(d[0].transpose(0, 1), 4),
+    lambda b, d: b.rotation(d[0][0, 0].float(), None, None, 1, False), lambda b, d: b.table_map(d[3], 1 << 40, 16)])
+def test_refusals_of_tensors(dev, call):
+    from voidinfer_amd import _binding
+    data = (torch.zeros(7, 4, 16, 64, dtype=torch.bfloat16, device=dev), torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev),
+            torch.zeros(6, dtype=torch.int32, device=dev), torch.zeros(5, 9, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError):
+        call(_binding, data)

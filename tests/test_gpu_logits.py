@@ -262,6 +262,7 @@ def test_refusals_on_the_device_side(dev):
 
 
 def test_masks_in_host_memory_are_refused(dev):
+    import voidinfer_amd as vi
     x = torch.zeros(2, 64, device=dev)
     with pytest.raises(ValueError):
         vi.process_logits(x, masks=torch.zeros(1, 2, dtype=torch.int32), mask_index=torch.zeros(2, dtype=torch.int32, device=dev))

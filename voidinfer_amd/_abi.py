@@ -17,6 +17,7 @@ import os
 
 # VOIDINFER_AMD_LIB selects another build of the same library (e.g. an instrumented one).
 LIB_PATH = Path(os.environ.get("VOIDINFER_AMD_LIB", Path(__file__).resolve().parent / "libvoidinfer_sampling.so"))
+BINDING_PATH = Path(__file__).resolve().parent / "_binding.so"   # tensors to the host structs (csrc/binding.cpp)
 
 BF16, F16, F32 = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_LAUNCH, ERR_DEVICE = range(6)
@@ -58,8 +59,8 @@ class DeviceSampling(C.Structure):
 
 assert C.sizeof(DeviceSampling) == 40
 
-# Host structs of the logit rules and of the paged cache, packed once per call
-# (field order and padding as in the header).
+# Host structs of the logit rules and of the paged cache (field order and padding as in
+# the header); the calls on tensors pack all but the first in csrc/binding.cpp.
 LOGIT_RULES = struct.Struct("<12Qqiiii")     # vi_logit_rules
 KV_CACHE = struct.Struct("<2Q3qiiiiii")      # vi_kv_cache
 LANE_ROWS = struct.Struct("<3Qqiiii")        # vi_lane_rows
@@ -136,10 +137,11 @@ def load() -> C.CDLL:
     """Load the in-tree library (ImportError if it has not been built)."""
     global _lib
     if _lib is None:
-        if not LIB_PATH.exists():
-            raise ImportError(
-                f"{LIB_PATH} is missing: build it with `python voidinfer_amd/build.py` "
-                "(there is no CPU fallback)")
+        for path in (LIB_PATH, BINDING_PATH):
+            if not path.exists():
+                raise ImportError(
+                    f"{path} is missing: build it with `python voidinfer_amd/build.py` "
+                    "(there is no CPU fallback)")
         lib = C.CDLL(str(LIB_PATH))
         for name, (args, res) in SIGNATURES.items():
             try:

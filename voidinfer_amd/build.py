@@ -2,7 +2,8 @@
 
 ``python voidinfer_amd/build.py`` (or ``build()``) compiles every HIP source
 under ``voidinfer_amd/csrc`` with hipcc for gfx950 and links
-``voidinfer_amd/libvoidinfer_sampling.so``.  Objects go to ``_build/``.  Run it as a
+``voidinfer_amd/libvoidinfer_sampling.so``, and builds ``voidinfer_amd/_binding.so``
+(how Python's tensors reach it).  Objects go to ``_build/``.  Run it as a
 script (not ``-m``): importing the package loads the library this builds.
 """
 from __future__ import annotations
@@ -19,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libvoidinfer_sampling.so"
+BINDING = PKG / "_binding.so"
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 
@@ -50,8 +52,10 @@ def _compile(src: Path) -> Path:
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = sources()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        binding = ex.submit(build_binding, verbose)
         objs = list(ex.map(_compile, srcs))
+        binding.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -62,6 +66,27 @@ def build(verbose: bool = False) -> Path:
         print(f"built {LIB}")
     build_launcher_test(verbose)
     return LIB
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """The Python module that packs tensors into the C ABI's structs (host code over torch's headers)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(x for p in (*include_paths(), sysconfig.get_paths()["include"]) for x in ("-isystem", p)),
+           str(CSRC / "binding.cpp"), "-o", str(tmp), "-L", str(Path(torch.__file__).parent / "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for binding.cpp:\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    if verbose:
+        print(f"built {BINDING}")
+    return BINDING
 
 
 # The compiled GPU test of the C++ launchers (tests/cpp/test_launchers_gpu.cpp):

@@ -24,47 +24,11 @@ import math
 
 import torch
 
-from . import _abi
 from ._abi import check
-from .ops import _int_list, _lib, _stream, workspace
-
+from ._binding import device_list, head_rows, kv_cache, lane_rows, page_map, page_pool, rotation, table_map
+from .ops import _lib, _stream, workspace
 
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
-_TYPES = {torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
-
-
-def _cache_args(k_pages: torch.Tensor, v_pages: torch.Tensor, shape: torch.Size) -> bytes:
-    strides, dtype = k_pages.stride(), k_pages.dtype
-    if len(shape) != 4 or shape != v_pages.shape or strides != v_pages.stride() or dtype is not v_pages.dtype:
-        raise ValueError("pages must be [pages, kv_heads, page_size, head_dim], keys and values alike")
-    if strides[3] != 1 or dtype not in _TYPES or not k_pages.is_cuda or not v_pages.is_cuda:
-        raise ValueError("pages must be bf16 or fp16 device memory with contiguous head_dim")
-    return _abi.KV_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], strides[2],
-                              _TYPES[dtype], shape[0], shape[2], shape[1], shape[3], 0)
-
-
-def _lane_args(tables: torch.Tensor, row_offsets: torch.Tensor, context: torch.Tensor, rows: int) -> bytes:
-    address, stride, lanes, width = _table_args(tables)
-    return _abi.LANE_ROWS.pack(_int_list(row_offsets, _I32, "row_offsets", lanes + 1),
-                               _int_list(context, _I32, "context", lanes), address, stride, width, lanes, rows, 0)
-
-
-def _table_args(tables: torch.Tensor) -> tuple[int, int, int, int]:
-    """(address, stride, lanes, width)"""
-    if tables.dtype is not _I32 or tables.dim() != 2 or not tables.is_cuda:
-        raise ValueError("tables must be int32 [lanes, pages per lane] device memory")
-    lanes, width = tables.shape
-    stride, one = tables.stride()
-    if one != 1 and width > 1:
-        raise ValueError("tables must have contiguous rows")
-    return tables.data_ptr(), stride if stride > width else width, lanes, width
-
-
-def _head_args(x: torch.Tensor, shape: tuple[int, int, int], dtype: torch.dtype, name: str) -> tuple[int, int, int]:
-    row, head, one = x.stride() if x.dim() == 3 else (0, 0, 0)
-    if one != 1 or x.dtype is not dtype or x.shape != shape or not x.is_cuda:
-        raise ValueError(f"{name} must be [rows, heads, head_dim] of the pages' type, head_dim contiguous")
-    return x.data_ptr(), row, head
 
 
 def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
@@ -81,32 +45,21 @@ def norm_rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     [angle rows, rotary / 2] or None (no rotation), row positions[r] (int32
     [rows]; default: the row's cache index).  A weight of None: no norm.  flags:
     int32 [rows], VI_FLAG_ERROR on rows that could not be placed."""
-    shape, dtype = k_pages.shape, k_pages.dtype
-    cache = _cache_args(k_pages, v_pages, shape)
-    kv_heads, dim = shape[1], shape[3]
+    cache = kv_cache(k_pages, v_pages)
+    _, kv_heads, _, dim = k_pages.shape
     rows, heads = q.shape[0], q.shape[1]
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
-    rotary = angle_rows = ca = sa = 0
-    if cosines is not None:
-        if sines is None or cosines.dtype is not _F32 or sines.dtype is not _F32 or cosines.dim() != 2 or \
-                cosines.shape != sines.shape or not cosines.is_contiguous() or not sines.is_contiguous() or \
-                not cosines.is_cuda or not sines.is_cuda:
-            raise ValueError("cosines and sines must be contiguous fp32 [angle rows, rotary / 2] device tensors")
-        angle_rows, rotary = cosines.shape
-        rotary, ca, sa = 2 * rotary, cosines.data_ptr(), sines.data_ptr()
-    elif sines is not None:
-        raise ValueError("sines need cosines")
-    qa, oa = _head_args(q, (rows, heads, dim), dtype, "q"), _head_args(out, (rows, heads, dim), dtype, "out")
+    dtype = k_pages.dtype
+    qa = head_rows(q, rows, heads, dim, k_pages, "q")
+    head_rows(out, rows, heads, dim, k_pages, "out")
     check(_lib().vi_norm_rotate_append(
-        cache, _lane_args(tables, row_offsets, context, rows), heads, _abi.HEAD_ROWS.pack(*qa),
-        _abi.HEAD_ROWS.pack(*_head_args(k, (rows, kv_heads, dim), dtype, "k")),
-        _abi.HEAD_ROWS.pack(*_head_args(v, (rows, kv_heads, dim), dtype, "v")),
-        None if q_weight is None else _int_list(q_weight, dtype, "q_weight", dim),
-        None if k_weight is None else _int_list(k_weight, dtype, "k_weight", dim), eps,
-        _abi.ROTATION.pack(ca, sa, 0 if positions is None else _int_list(positions, _I32, "positions", rows),
-                           angle_rows, rotary, interleaved, 0),
-        *oa, None if flags is None else _int_list(flags, _I32, "flags", rows), _stream()), "vi_norm_rotate_append")
+        cache, lane_rows(tables, row_offsets, context, rows), heads, qa,
+        head_rows(k, rows, kv_heads, dim, k_pages, "k"), head_rows(v, rows, kv_heads, dim, k_pages, "v"),
+        None if q_weight is None else device_list(q_weight, dtype, "q_weight", dim),
+        None if k_weight is None else device_list(k_weight, dtype, "k_weight", dim), eps,
+        rotation(cosines, sines, positions, rows, interleaved), out.data_ptr(), out.stride(0), out.stride(1),
+        None if flags is None else device_list(flags, _I32, "flags", rows), _stream()), "vi_norm_rotate_append")
     return out
 
 
@@ -126,9 +79,8 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     max_own: bounds of a lane's rows, and of its tokens past the shared prefix;
     max_group_rows / max_prefix: the same of a group.  scale: 1 / sqrt(d) unless
     given.  lse: fp32 [rows, heads], written when given."""
-    shape, dtype = k_pages.shape, k_pages.dtype
-    cache = _cache_args(k_pages, v_pages, shape)
-    kv_heads, dim = shape[1], shape[3]
+    cache = kv_cache(k_pages, v_pages)
+    _, kv_heads, _, dim = k_pages.shape
     rows, heads = q.shape[0], q.shape[1]
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
@@ -137,51 +89,36 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         if prefix_lens is None:
             raise ValueError("group_offsets need prefix_lens")
         groups = prefix_lens.numel()
-        go, pl = _int_list(group_offsets, _I32, "group_offsets", groups + 1), _int_list(prefix_lens, _I32, "prefix_lens")
+        go = device_list(group_offsets, _I32, "group_offsets", groups + 1)
+        pl = device_list(prefix_lens, _I32, "prefix_lens", None)
     if lse is not None and (lse.dtype is not _F32 or lse.shape != (rows, heads) or not lse.is_contiguous() or
                             not lse.is_cuda):
         raise ValueError("lse must be contiguous fp32 [rows, heads]")
-    qa, oa = _head_args(q, (rows, heads, dim), dtype, "q"), _head_args(out, (rows, heads, dim), dtype, "out")
-    lanes = _lane_args(tables, row_offsets, context, rows)
+    qa = head_rows(q, rows, heads, dim, k_pages, "q")
+    head_rows(out, rows, heads, dim, k_pages, "out")
+    lanes = lane_rows(tables, row_offsets, context, rows)
     lib, stream = _lib(), _stream()
     nb = lib.vi_prefix_attention_workspace_bytes(rows, heads, kv_heads, dim, tables.shape[0], groups, max_rows,
                                                  max_group_rows, max_own, max_prefix)
     ws = workspace(("attention", stream), nb, q.device)
     check(lib.vi_prefix_attention(
-        cache, lanes, heads, _abi.HEAD_ROWS.pack(*qa), 1.0 / math.sqrt(dim) if scale is None else scale, groups, go,
-        pl, max_rows, max_group_rows, max_own, max_prefix,
-        None if tree is None else _int_list(tree, _I64, "tree", rows), *oa,
-        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream), "vi_prefix_attention")
+        cache, lanes, heads, qa, 1.0 / math.sqrt(dim) if scale is None else scale, groups, go, pl, max_rows,
+        max_group_rows, max_own, max_prefix, None if tree is None else device_list(tree, _I64, "tree", rows),
+        out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        stream), "vi_prefix_attention")
     return out
-
-
-def _map_args(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor | None, page_size: int,
-              status: torch.Tensor | None) -> bytes:
-    address, stride, lanes, width = _table_args(tables)
-    return _abi.PAGE_MAP.pack(_int_list(refs, _I32, "refs"), address,
-                              0 if lengths is None else _int_list(lengths, _I32, "lengths", lanes),
-                              0 if status is None else _int_list(status, _I32, "status", 3), stride, refs.numel(),
-                              page_size, lanes, width)
-
-
-def _pool_args(pool: torch.Tensor, pages: int) -> bytes:
-    if pool.dim() < 4 or not pool.is_cuda or not pool.is_contiguous() or pool.shape[-4] != pages:
-        raise ValueError("pool must be contiguous [..., pages, kv_heads, page_size, head_dim] device memory")
-    elements = pool.stride(-4)
-    page_bytes = elements * pool.element_size()
-    return _abi.PAGE_POOL.pack(pool.data_ptr(), page_bytes * pages, page_bytes, pool.numel() // (elements * pages), 0)
 
 
 def _pair(a: torch.Tensor, b: torch.Tensor, names: tuple[str, str]) -> tuple[int, int, int]:
     n = a.numel()
-    return _int_list(a, _I32, names[0]), _int_list(b, _I32, names[1], n), n
+    return device_list(a, _I32, names[0], None), device_list(b, _I32, names[1], n), n
 
 
 def pages_fork(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor,
                children: torch.Tensor, page_size: int, status: torch.Tensor | None = None) -> None:
     """children[i] (int32 lanes) gives back its pages and shares parents[i]'s (vi_pages_fork)."""
     a, b, n = _pair(parents, children, ("parents", "children"))
-    check(_lib().vi_pages_fork(_map_args(refs, tables, lengths, page_size, status), a, b, n, _stream()),
+    check(_lib().vi_pages_fork(page_map(refs, tables, lengths, page_size, status), a, b, n, _stream()),
           "vi_pages_fork")
 
 
@@ -192,7 +129,7 @@ def pages_extend(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tensor
     a, b, n = _pair(lanes, new_lengths, ("lanes", "new_lengths"))
     lib, stream = _lib(), _stream()
     ws = workspace(("pages", stream), lib.vi_pages_extend_workspace_bytes(n), refs.device)
-    check(lib.vi_pages_extend(_map_args(refs, tables, lengths, pool.shape[-2], status), _pool_args(pool, refs.numel()),
+    check(lib.vi_pages_extend(page_map(refs, tables, lengths, pool.shape[-2], status), page_pool(pool, refs.numel()),
                               a, b, n, ws.data_ptr(), ws.numel(), stream), "vi_pages_extend")
 
 
@@ -200,7 +137,7 @@ def pages_truncate(refs: torch.Tensor, tables: torch.Tensor, lengths: torch.Tens
                    new_lengths: torch.Tensor, page_size: int, status: torch.Tensor | None = None) -> None:
     """lanes[i] shrinks to new_lengths[i] tokens, 0 frees it (vi_pages_truncate)."""
     a, b, n = _pair(lanes, new_lengths, ("lanes", "new_lengths"))
-    check(_lib().vi_pages_truncate(_map_args(refs, tables, lengths, page_size, status), a, b, n, _stream()),
+    check(_lib().vi_pages_truncate(page_map(refs, tables, lengths, page_size, status), a, b, n, _stream()),
           "vi_pages_truncate")
 
 
@@ -208,7 +145,7 @@ def pages_copy(pool: torch.Tensor, sources: torch.Tensor, targets: torch.Tensor)
     """Page sources[i] to page targets[i] in every plane of the pool (vi_pages_copy)."""
     a, b, n = _pair(sources, targets, ("sources", "targets"))
     pages = pool.shape[-4]
-    check(_lib().vi_pages_copy(_pool_args(pool, pages), pages, a, b, n, _stream()), "vi_pages_copy")
+    check(_lib().vi_pages_copy(page_pool(pool, pages), pages, a, b, n, _stream()), "vi_pages_copy")
 
 
 def pages_compact(refs: torch.Tensor, tables: torch.Tensor, pool: torch.Tensor,
@@ -218,7 +155,7 @@ def pages_compact(refs: torch.Tensor, tables: torch.Tensor, pool: torch.Tensor,
     lib, stream = _lib(), _stream()
     ws = workspace(("pages", stream), lib.vi_pages_compact_workspace_bytes(refs.numel()), refs.device)
     # (a compaction needs no lengths: the tables say what is held)
-    check(lib.vi_pages_compact(_map_args(refs, tables, None, pool.shape[-2], status), _pool_args(pool, refs.numel()),
+    check(lib.vi_pages_compact(page_map(refs, tables, None, pool.shape[-2], status), page_pool(pool, refs.numel()),
                                ws.data_ptr(), ws.numel(), stream), "vi_pages_compact")
 
 
@@ -230,9 +167,8 @@ def keep_rows(pool: torch.Tensor, tables: torch.Tensor, lanes: torch.Tensor, con
     if paths.dtype is not _I32 or paths.dim() != 2 or paths.shape[0] != n or not paths.is_contiguous() or \
             not paths.is_cuda:
         raise ValueError("paths must be contiguous int32 [lanes, width] device memory")
-    address, stride, count, width = _table_args(tables)
     pages, kv_heads, page_size, _ = pool.shape[-4:]
     check(_lib().vi_keep_rows(
-        _abi.PAGE_MAP.pack(0, address, 0, 0, stride, pages, page_size, count, width), _pool_args(pool, pages), kv_heads,
-        _int_list(lanes, _I32, "lanes"), _int_list(context, _I32, "context", n), paths.data_ptr(), paths.shape[1],
-        _int_list(kept, _I32, "kept", n), n, _stream()), "vi_keep_rows")
+        table_map(tables, pages, page_size), page_pool(pool, pages), kv_heads, device_list(lanes, _I32, "lanes", None),
+        device_list(context, _I32, "context", n), paths.data_ptr(), paths.shape[1], device_list(kept, _I32, "kept", n), n,
+        _stream()), "vi_keep_rows")

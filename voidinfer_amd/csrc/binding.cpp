@@ -1,0 +1,202 @@
+// binding.cpp — tensors to the C ABI's host structs (the module voidinfer_amd._binding).
+//
+// A call on a paged cache takes a dozen tensors; checked and read from Python, one
+// attribute at a time, they cost more than the launch and most of the kernels of a
+// small call: norm_rotate_append 8.1 us of host time without the launch, 2.3 so (a
+// call of 8 rows 12.9 -> 7.8 us, attention of 4 rows 15.9 -> 12.8).  Here each struct's
+// tensors are checked and packed in one function.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstdint>
+
+#include "../../include/voidinfer_sampling.h"
+
+namespace {
+
+struct Refused {};   // the Python error is set
+
+[[noreturn]] void refuse(const char* text) {
+    PyErr_SetString(PyExc_ValueError, text);
+    throw Refused{};
+}
+const at::Tensor& tensor(PyObject* o, const char* what) {
+    if (!THPVariable_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "%s must be a tensor", what);
+        throw Refused{};
+    }
+    return THPVariable_Unpack(o);
+}
+int64_t whole(PyObject* o) {
+    const long long x = PyLong_AsLongLong(o);
+    if (x == -1 && PyErr_Occurred()) throw Refused{};
+    return x;
+}
+void arguments(Py_ssize_t n, Py_ssize_t want) {
+    if (n == want) return;
+    PyErr_Format(PyExc_TypeError, "%zd arguments instead of %zd", n, want);
+    throw Refused{};
+}
+template <class T> PyObject* bytes(const T& x) {
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&x), sizeof(T));
+}
+
+// A contiguous 1-d device list of a type, with `count` entries where that is not negative.
+void* list_of(PyObject* o, at::ScalarType type, const char* name, int64_t count) {
+    const at::Tensor& t = tensor(o, name);
+    if (t.scalar_type() != type || t.dim() != 1 || !t.is_cuda() || !t.is_contiguous()) {
+        PyErr_Format(PyExc_ValueError, "%s must be a contiguous 1-d device tensor of torch.%s", name,
+                     type == at::kInt ? "int32" : type == at::kLong ? "int64" : type == at::kFloat ? "float32" :
+                     type == at::kBFloat16 ? "bfloat16" : type == at::kHalf ? "float16" : "another type");
+        throw Refused{};
+    }
+    if (count >= 0 && t.numel() != count) {
+        PyErr_Format(PyExc_ValueError, "%s must have %lld entries", name, static_cast<long long>(count));
+        throw Refused{};
+    }
+    return t.data_ptr();
+}
+int32_t* int_list(PyObject* o, const char* name, int64_t count) {   // None: NULL
+    return o == Py_None ? nullptr : static_cast<int32_t*>(list_of(o, at::kInt, name, count));
+}
+
+struct Table {
+    int32_t* address;
+    int64_t stride, lanes, width;
+};
+Table table(PyObject* o) {
+    const at::Tensor& t = tensor(o, "tables");
+    if (t.scalar_type() != at::kInt || t.dim() != 2 || !t.is_cuda())
+        refuse("tables must be int32 [lanes, pages per lane] device memory");
+    if (t.stride(1) != 1 && t.size(1) > 1) refuse("tables must have contiguous rows");
+    return {static_cast<int32_t*>(t.data_ptr()), t.stride(0) > t.size(1) ? t.stride(0) : t.size(1), t.size(0), t.size(1)};
+}
+int32_t small(int64_t x) {
+    if (x < INT32_MIN || x > INT32_MAX) refuse("a size does not fit 32 bits");
+    return int32_t(x);
+}
+
+// device_list(t, dtype, name, count or None) -> address
+PyObject* device_list(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 4);
+    if (!THPDtype_Check(a[1])) refuse("a dtype is needed");
+    const char* const name = PyUnicode_AsUTF8(a[2]);
+    if (!name) throw Refused{};
+    return PyLong_FromVoidPtr(list_of(a[0], reinterpret_cast<THPDtype*>(a[1])->scalar_type, name,
+                                      a[3] == Py_None ? -1 : whole(a[3])));
+}
+
+// kv_cache(k_pages, v_pages) -> vi_kv_cache
+PyObject* kv_cache(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 2);
+    const at::Tensor &k = tensor(a[0], "k_pages"), &v = tensor(a[1], "v_pages");
+    if (k.dim() != 4 || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type())
+        refuse("pages must be [pages, kv_heads, page_size, head_dim], keys and values alike");
+    if (k.stride(3) != 1 || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf) || !k.is_cuda() || !v.is_cuda())
+        refuse("pages must be bf16 or fp16 device memory with contiguous head_dim");
+    return bytes(vi_kv_cache{k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                             k.scalar_type() == at::kBFloat16 ? VI_BF16 : VI_F16, small(k.size(0)), small(k.size(2)),
+                             small(k.size(1)), small(k.size(3)), 0});
+}
+
+// lane_rows(tables, row_offsets, context, rows) -> vi_lane_rows
+PyObject* lane_rows(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 4);
+    const Table t = table(a[0]);
+    return bytes(vi_lane_rows{static_cast<int32_t*>(list_of(a[1], at::kInt, "row_offsets", t.lanes + 1)),
+                              static_cast<int32_t*>(list_of(a[2], at::kInt, "context", t.lanes)), t.address, t.stride,
+                              small(t.width), small(t.lanes), small(whole(a[3])), 0});
+}
+
+// head_rows(x, rows, heads, head_dim, pages, name) -> vi_head_rows; x of the pages' type
+PyObject* head_rows(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 6);
+    const char* const name = PyUnicode_AsUTF8(a[5]);
+    if (!name) throw Refused{};
+    const at::Tensor &x = tensor(a[0], name), &pages = tensor(a[4], "pages");
+    if (x.dim() != 3 || x.stride(2) != 1 || x.scalar_type() != pages.scalar_type() || x.size(0) != whole(a[1]) ||
+        x.size(1) != whole(a[2]) || x.size(2) != whole(a[3]) || !x.is_cuda()) {
+        PyErr_Format(PyExc_ValueError, "%s must be [rows, heads, head_dim] of the pages' type, head_dim contiguous", name);
+        throw Refused{};
+    }
+    return bytes(vi_head_rows{x.data_ptr(), x.stride(0), x.stride(1)});
+}
+
+// rotation(cosines or None, sines or None, positions or None, rows, interleaved) -> vi_rotation
+PyObject* rotation(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 5);
+    vi_rotation r{};
+    if (a[0] != Py_None) {
+        const at::Tensor& c = tensor(a[0], "cosines");
+        const at::Tensor* const s = a[1] == Py_None ? nullptr : &tensor(a[1], "sines");
+        if (!s || c.scalar_type() != at::kFloat || s->scalar_type() != at::kFloat || c.dim() != 2 || c.sizes() != s->sizes() ||
+            !c.is_contiguous() || !s->is_contiguous() || !c.is_cuda() || !s->is_cuda())
+            refuse("cosines and sines must be contiguous fp32 [angle rows, rotary / 2] device tensors");
+        r.cosines = static_cast<const float*>(c.data_ptr());
+        r.sines = static_cast<const float*>(s->data_ptr());
+        r.angle_rows = small(c.size(0));
+        r.rotary_dim = small(2 * c.size(1));
+    } else if (a[1] != Py_None) {
+        refuse("sines need cosines");
+    }
+    r.positions = int_list(a[2], "positions", whole(a[3]));
+    const int interleaved = PyObject_IsTrue(a[4]);
+    if (interleaved < 0) throw Refused{};
+    r.interleaved = interleaved;
+    return bytes(r);
+}
+
+// page_map(refs, tables, lengths or None, page_size, status or None) -> vi_page_map
+PyObject* page_map(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 5);
+    const Table t = table(a[1]);
+    int32_t* const refs = static_cast<int32_t*>(list_of(a[0], at::kInt, "refs", -1));
+    return bytes(vi_page_map{refs, t.address, int_list(a[2], "lengths", t.lanes), int_list(a[4], "status", 3), t.stride,
+                             small(THPVariable_Unpack(a[0]).numel()), small(whole(a[3])), small(t.lanes), small(t.width)});
+}
+// table_map(tables, pages, page_size) -> vi_page_map of a call that needs the tables alone
+PyObject* table_map(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 3);
+    const Table t = table(a[0]);
+    return bytes(vi_page_map{nullptr, t.address, nullptr, nullptr, t.stride, small(whole(a[1])), small(whole(a[2])),
+                             small(t.lanes), small(t.width)});
+}
+
+// page_pool(pool, pages) -> vi_page_pool
+PyObject* page_pool(PyObject* const* a, Py_ssize_t n) {
+    arguments(n, 2);
+    const at::Tensor& p = tensor(a[0], "pool");
+    const int64_t pages = whole(a[1]);
+    if (p.dim() < 4 || !p.is_cuda() || !p.is_contiguous() || p.size(-4) != pages)
+        refuse("pool must be contiguous [..., pages, kv_heads, page_size, head_dim] device memory");
+    const int64_t elements = p.size(-3) * p.size(-2) * p.size(-1), page = elements * p.element_size();
+    return bytes(vi_page_pool{p.data_ptr(), page * pages, page, small(elements * pages ? p.numel() / (elements * pages) : 0), 0});
+}
+
+template <PyObject* (*kFn)(PyObject* const*, Py_ssize_t)> PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    try {
+        return kFn(a, n);
+    } catch (const Refused&) {
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "unknown error");
+    }
+    return nullptr;
+}
+template <PyObject* (*kFn)(PyObject* const*, Py_ssize_t)> PyMethodDef method(const char* name) {
+    return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&entry<kFn>)), METH_FASTCALL, nullptr};
+}
+
+PyMethodDef methods[] = {
+    method<device_list>("device_list"), method<kv_cache>("kv_cache"), method<lane_rows>("lane_rows"),
+    method<head_rows>("head_rows"), method<rotation>("rotation"), method<page_map>("page_map"),
+    method<table_map>("table_map"), method<page_pool>("page_pool"), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__binding() { return PyModule_Create(&module); }

@@ -30,6 +30,7 @@ import torch
 
 from . import _abi
 from ._abi import (BF16, F16, F32, GREEDY_ROW, ROW_PARAMS, SAMPLE_STATS, DeviceSampling, check)
+from ._binding import device_list
 
 _DTYPES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 _workspaces: dict[tuple, torch.Tensor] = {}
@@ -390,15 +391,6 @@ def sample_rows_state(logits: torch.Tensor, params: np.ndarray | torch.Tensor, s
     return o
 
 
-def _int_list(t: torch.Tensor, dtype: torch.dtype, name: str, count: int | None = None) -> int:
-    """Address of a contiguous 1-d device list of `dtype` (with `count` entries, where that is given)."""
-    if t.dtype is not dtype or t.dim() != 1 or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous 1-d device tensor of {dtype}")
-    if count is not None and t.numel() != count:
-        raise ValueError(f"{name} must have {count} entries")
-    return t.data_ptr()
-
-
 def process_logits(logits: torch.Tensor, params: np.ndarray | torch.Tensor | None = None, *,
                    lanes: torch.Tensor | None = None, histories: torch.Tensor | None = None,
                    offsets: torch.Tensor | None = None, state: PenaltyState | None = None,
@@ -436,12 +428,12 @@ def process_logits(logits: torch.Tensor, params: np.ndarray | torch.Tensor | Non
     n_lanes = n_lanes or next((t.numel() - 1 for t in lists if t is not None), rows)
     if any(t is not None and t.numel() != n_lanes + 1 for t in lists):
         raise ValueError("offsets and bias_offsets must have lanes + 1 entries")
-    row_lanes = 0 if lanes is None else _int_list(lanes, torch.int32, "lanes", rows)
+    row_lanes = 0 if lanes is None else device_list(lanes, torch.int32, "lanes", rows)
     h = ho = e = eo = bi = bv = bo = m = mi = stride_m = n_masks = st = slots = 0
     if histories is not None:
         if offsets is None or state is not None:
             raise ValueError("histories need offsets and exclude a penalty state")
-        h, ho = _int_list(histories, torch.int32, "histories"), _int_list(offsets, torch.int64, "offsets")
+        h, ho = device_list(histories, torch.int32, "histories", None), device_list(offsets, torch.int64, "offsets", None)
     if state is not None:
         if n_lanes > state.lanes or vocab != state.vocabulary:
             raise ValueError("penalty state has too few lanes or another vocabulary")
@@ -449,23 +441,23 @@ def process_logits(logits: torch.Tensor, params: np.ndarray | torch.Tensor | Non
     if extra is not None:
         if extra_offsets is None:
             raise ValueError("extra needs extra_offsets")
-        e = _int_list(extra, torch.int32, "extra")
-        eo = _int_list(extra_offsets, torch.int64, "extra_offsets", rows + 1)
+        e = device_list(extra, torch.int32, "extra", None)
+        eo = device_list(extra_offsets, torch.int64, "extra_offsets", rows + 1)
     if bias_ids is not None:
         if bias_values is None or bias_offsets is None:
             raise ValueError("bias_ids need bias_values and bias_offsets")
-        bi = _int_list(bias_ids, torch.int32, "bias_ids")
-        bv = _int_list(bias_values, torch.float32, "bias_values", bias_ids.numel())
-        bo = _int_list(bias_offsets, torch.int64, "bias_offsets")
+        bi = device_list(bias_ids, torch.int32, "bias_ids", None)
+        bv = device_list(bias_values, torch.float32, "bias_values", bias_ids.numel())
+        bo = device_list(bias_offsets, torch.int64, "bias_offsets", None)
     if mask_index is not None:
         if masks is None or masks.dtype != torch.int32 or masks.dim() != 2 or masks.stride(1) != 1 or \
                 masks.shape[1] * 32 < vocab or not masks.is_cuda:
             raise ValueError("masks must be int32 [n, ceil(vocabulary / 32)] device memory with contiguous rows")
-        mi = _int_list(mask_index, torch.int32, "mask_index", rows)
+        mi = device_list(mask_index, torch.int32, "mask_index", rows)
         m, n_masks, stride_m = masks.data_ptr(), masks.shape[0], max(masks.stride(0), masks.shape[1])
     elif masks is not None:
         raise ValueError("masks need mask_index")
-    f = 0 if flags is None else _int_list(flags, torch.int32, "flags", rows)
+    f = 0 if flags is None else device_list(flags, torch.int32, "flags", rows)
     rules = _abi.LOGIT_RULES.pack(p_ptr, row_lanes, h, ho, st, e, eo, bi, bv, bo, m, mi, stride_m, n_lanes, n_masks,
                                   slots, 0)
     check(_lib().vi_process_logits(logits.data_ptr(), dtype, rows, vocab, stride, rules, out.data_ptr(), out_stride,
