@@ -277,6 +277,20 @@ def test_copy_past_32_bits(dev):
     assert pool[0, pages - 2, 0, 0, 0] == 5 and not pool[0, 2].any() and not pool[0, pages - 3].any()
 
 
+@pytest.mark.parametrize("rows,dim", [(255, 8), (257, 24), (700, 64)])
+def test_long_paths(dev, rng, rows, dim):
+    """More rows than a workgroup looks up at once, and more vectors than it holds, moving over page ends."""
+    m = Model(2, 80, 170, 16, 2, 3, dim, rng)
+    d = Device(m, dev)
+    m.extend([0, 1], [37 + rows + 500, 20])
+    d.extend([0, 1], [37 + rows + 500, 20])
+    path = np.sort(rng.permutation(np.arange(1, rows + 480))[:rows - 3])
+    path = [0, 1, 2] + [int(x) + 2 for x in path]
+    m.keep([0, 1], [37, 5], [path, path], [len(path), 1])
+    d.keep([0, 1], [37, 5], [path, path], [len(path), 1])
+    same(m, d, "keep")
+
+
 def test_paths_that_are_not_so(dev, rng):
     """Entries that do not ascend, stand before their place or lead outside the lane's pages are skipped; the
     others move."""

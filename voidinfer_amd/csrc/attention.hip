@@ -712,8 +712,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     const int kv = int(blockIdx.x / (D / 32) % unsigned(a.cache.kv_heads));
     const int64_t query = int64_t(blockIdx.x / (D / 32) / unsigned(a.cache.kv_heads)) * 32 + threadIdx.x % 32;
     const int row = int(query / per_kv), g = int(query % per_kv), head = kv * per_kv + g;
+    RowInfo r = a.info[min(row, a.lanes.rows - 1)];   // (requested beside the number of rows)
+    asm volatile("" ::: "memory");
     if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
-    RowInfo r = a.info[row];
     // (a row that no lane holds, of offsets that do not begin at 0 or fall, has whatever lay there)
     r.own_parts = min(r.own_parts, a.plan.own.splits);
     r.group_parts = min(r.group_parts, r.group < 0 ? 0 : a.plan.prefix.splits);

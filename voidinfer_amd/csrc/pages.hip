@@ -9,7 +9,7 @@
 // nothing waits for the host.
 //
 // The plans are bound by their dependent reads, the copies by memory.  Over 2,048
-// pages: extend's plan of 64 lanes 8.4 us, of 16 8.6; compact's 4.8 us; fork of 12
+// pages: extend's plan of 64 lanes 6.1 us, of 16 6.6; compact's 4.8 us; fork of 12
 // lanes 3.4, truncate of 64 3.2.  Compact's copy of 784 MB: 322 us, 4.9 TB/s read and
 // written together, the rate of a plain copy.
 #include <algorithm>
@@ -181,13 +181,18 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
     if (tid == 0) large = 0;
     __syncthreads();
 
-    int lane[kListPer], held[kListPer], need[kListPer], last[kListPer], length[kListPer];
+    // A thread's entries of the list, neighbours: one as long as the threads suffice (each is
+    // a chain of four reads, and a thread's chains follow one another: 64 lanes with
+    // four entries a thread took 8.3 us)
+    const int per = (count + kPlan - 1) / kPlan;
+    auto entry = [&](int k) { return k < per ? tid * per + k : count; };
+    int lane[kListPer], held[kListPer], need[kListPer], last[kListPer], length[kListPer], holders[kListPer];
     uint32_t slot[kListPer];
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < kListPer; ++k) {
-        const int i = tid * kListPer + k;
-        lane[k] = -1; held[k] = need[k] = 0; last[k] = -1; length[k] = 0; slot[k] = 0u;
+        const int i = entry(k);
+        lane[k] = -1; held[k] = need[k] = 0; last[k] = -1; length[k] = 0; slot[k] = 0u; holders[k] = 0;
         if (i >= count) continue;
         const int l = lane_ids[i], to = new_lengths[i];
         if (uint32_t(l) >= uint32_t(m.lanes)) { bad = true; continue; }
@@ -201,7 +206,8 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
         if (now % m.page_size && to > now) {
             const int page = m.tables[int64_t(l) * m.table_stride + held[k] - 1];
             if (uint32_t(page) >= uint32_t(m.pages)) { bad = true; continue; }
-            if (m.refs[page] > 1) {
+            holders[k] = m.refs[page];
+            if (holders[k] > 1) {
                 last[k] = page;
                 uint32_t s = (uint32_t(page) * 0x9E3779B1u) >> shift;
                 for (;;) {   // (at most count keys in twice as many slots)
@@ -220,9 +226,9 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
     bool copied[kListPer];
 #pragma unroll
     for (int k = 0; k < kListPer; ++k) {
-        const int i = tid * kListPer + k;
+        const int i = entry(k);
         // the last listed lane keeps the page when the listed ones are all that hold it
-        copied[k] = last[k] >= 0 && !(uint32_t(m.refs[last[k]]) == sharers[slot[k]] && lasts[slot[k]] == uint32_t(i));
+        copied[k] = last[k] >= 0 && !(uint32_t(holders[k]) == sharers[slot[k]] && lasts[slot[k]] == uint32_t(i));
         need[k] += copied[k];
         mine += uint32_t(need[k]);
         copies += copied[k];
@@ -247,7 +253,7 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
     }
 #pragma unroll
     for (int k = 0; k < kListPer; ++k) {
-        const int i = tid * kListPer + k;
+        const int i = entry(k);
         if (i < count) base[i] = at;
         at += uint32_t(need[k]);
         if (copied[k]) {   // its copy's target follows below
@@ -270,7 +276,7 @@ __global__ __launch_bounds__(kPlan) void extend_kernel(vi_page_map m, const int3
     pair -= copies;
 #pragma unroll
     for (int k = 0; k < kListPer; ++k) {
-        const int i = tid * kListPer + k;
+        const int i = entry(k);
         if (i >= count) continue;
         info[i] = uint32_t(held[k]) << 1 | uint32_t(copied[k]);
         who[i] = lane[k];
@@ -393,8 +399,10 @@ constexpr int kKeepBatch = 4;   // vectors a thread holds between the reads and 
 // One workgroup per (lane, plane).  Rows move towards the front of an ascending
 // path, so batches in path order never overwrite a row that is still to be
 // read; within a batch every read comes before every write.  64 lanes x 32 planes
-// whose paths leave the chain once at the end: 19 us, reads that wait for one
-// another (list, path, table, row) in rows of 256 bytes all over the pool.
+// whose paths leave the chain once at the end: 6.5 us, of which 3 until the path is
+// known to move and the rest table, row and write, one behind the other; 16 rows of
+// each lane that move, 134 MB both ways: 29 us, 4.6 TB/s.  (With each thread's look-ups
+// beside its vectors 19 and 50 us.)
 __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     const int i = int(blockIdx.x / uint32_t(a.pool.planes)), plane = int(blockIdx.x % uint32_t(a.pool.planes)), tid = threadIdx.x;
     const int lane = a.lane_ids[i];
@@ -406,13 +414,11 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     if (context < 0) return;
     unsigned char* const base = static_cast<unsigned char*>(a.pool.base) + int64_t(plane) * a.pool.plane_stride;
     const int shift = __builtin_ctz(unsigned(a.m.page_size));
-    auto place = [&](int64_t index, uint32_t head, uint32_t vec) -> uint4* {
+    auto place = [&](int64_t index) -> int64_t {   // a token's row of head 0, in vectors; -1: no page
         const int64_t e = index >> shift;
-        if (e >= a.m.table_width) return nullptr;
-        const int page = table[e];
-        if (uint32_t(page) >= uint32_t(a.m.pages)) return nullptr;
-        return reinterpret_cast<uint4*>(base + int64_t(page) * a.pool.page_bytes) +
-               ((head << shift) + (uint32_t(index) & uint32_t(a.m.page_size - 1))) * uint32_t(a.vecs) + vec;
+        const int page = e < a.m.table_width ? table[e] : -1;
+        if (uint32_t(page) >= uint32_t(a.m.pages)) return -1;
+        return int64_t(page) * (a.pool.page_bytes / 16) + (uint32_t(index) & uint32_t(a.m.page_size - 1)) * uint32_t(a.vecs);
     };
     // rows that stay in place need nothing: the first that moves, found by all threads at once
     __shared__ int first_move;
@@ -426,27 +432,37 @@ __global__ __launch_bounds__(kKeepThreads) void keep_kernel(KeepArgs a) {
     __syncthreads();
     const int j0 = first_move;
     if (j0 >= n) return;
-    const uint32_t items = uint32_t(n - j0) * per_row;
-    for (uint32_t b = 0; b < items; b += kKeepThreads * kKeepBatch) {
-        uint4 v[kKeepBatch];
-        uint4* to[kKeepBatch];
-#pragma unroll
-        for (int k = 0; k < kKeepBatch; ++k) {
-            const uint32_t it = b + k * kKeepThreads + tid;
-            to[k] = nullptr;
-            if (it >= items) continue;
-            const uint32_t row = it / per_row, in = it - row * per_row, head = in / uint32_t(a.vecs), vec = in - head * uint32_t(a.vecs);
-            const int j = j0 + int(row), from = path[j];
-            if (from <= j || from >= 65536 || (j > 0 && path[j - 1] >= from)) continue;
-            const uint4* const src = place(int64_t(context) + from, head, vec);
-            to[k] = place(int64_t(context) + j, head, vec);
-            if (src && to[k]) v[k] = *src; else to[k] = nullptr;
+    // a thread looks up a row (-1: it does not move), then all copy
+    __shared__ int64_t source[kKeepThreads], target[kKeepThreads];
+    for (int r0 = j0; r0 < n; r0 += kKeepThreads) {
+        const int j = r0 + tid;
+        if (j < n) {
+            const int from = path[j], before = j > 0 ? path[j - 1] : -1;
+            const int64_t s = place(int64_t(context) + max(from, 0)), t = place(int64_t(context) + j);
+            const bool moves = from > j && from < 65536 && before < from && s >= 0 && t >= 0;
+            source[tid] = moves ? s : 0;   // (page 0 is read for it, and not used)
+            target[tid] = moves ? t : -1;
         }
         __syncthreads();
+        const uint32_t items = uint32_t(min(n - r0, kKeepThreads)) * per_row;
+        for (uint32_t b = 0; b < items; b += kKeepThreads * kKeepBatch) {
+            u32x4_t v[kKeepBatch];
+            int64_t to[kKeepBatch];
 #pragma unroll
-        for (int k = 0; k < kKeepBatch; ++k)
-            if (to[k]) *to[k] = v[k];
-        __syncthreads();
+            for (int k = 0; k < kKeepBatch; ++k) {
+                const uint32_t it = b + k * kKeepThreads + tid, in_range = min(it, items - 1);
+                const uint32_t row = in_range / per_row, in = in_range - row * per_row;
+                const uint32_t head = in / uint32_t(a.vecs), vec = in - head * uint32_t(a.vecs);
+                const int64_t o = int64_t((head << shift) * uint32_t(a.vecs) + vec);
+                v[k] = reinterpret_cast<const u32x4_t*>(base)[source[row] + o];
+                to[k] = it < items && target[row] >= 0 ? target[row] + o : -1;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kKeepBatch; ++k)
+                if (to[k] >= 0) reinterpret_cast<u32x4_t*>(base)[to[k]] = v[k];
+            __syncthreads();
+        }
     }
 }
 
