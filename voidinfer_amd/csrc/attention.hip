@@ -28,7 +28,7 @@
 // The matrix instructions of a wave's 32 queries need as much of LDS (each fragment
 // is read for 32 queries) as of the SIMD, and the softmax about as much of the
 // vector units; two workgroups a CU overlap these in part.  8 x 17 rows of 32 heads
-// over 4,096 shared and up to 1,500 own keys: 29 us, and 8 for the join (23 MB of parts).
+// over 4,096 shared and up to 1,500 own keys: 28 us, and 8 for the join (23 MB of parts).
 // 4 x 1 rows of 16 heads of 64 places over 512 and 100: 9 + 4 us, of which 5 the look-ups
 // before a part's first load (offsets, lengths, group, table, page).
 // Not taken: eight waves over 256 queries in step, one of a SIMD at the products while
@@ -600,7 +600,8 @@ __device__ __forceinline__ void attend_part(const AttnArgs& a, AttnLds<D>& lds, 
         const int64_t at = origin + int64_t(tile_of(i)) * kKeys;
         const int begin = int(max(k0 - at, int64_t(0))), end = int(min(k1 - at, int64_t(kKeys)));
         const int known = int(max(min(s.context - at, int64_t(kKeys)), int64_t(-(1 << 30))));
-        for (int b = 0; b < kMine; ++b) attend_masked(i % kStages, ki + b * kAlong, at, begin, end, known);
+        for (int b = ki; b < kBlocks && b * 32 < end; b += kAlong)   // (those behind the last key have nothing: 8 x 17 rows 36 us so, 38 with them)
+            if (b * 32 + 32 > begin) attend_masked(i % kStages, b, at, begin, end, known);
     }
 
     // the waves that shared queries join
