@@ -36,6 +36,7 @@
 // parts beside a prefix part); tiles of 32 keys four deep (160 to 214 us); prefix
 // and own parts launched alternately (the prefix alone 143 us).
 #include <algorithm>
+#include <cmath>
 
 #include "cache_rows.h"
 
@@ -705,17 +706,21 @@ __device__ __forceinline__ float4 no_numbers(const AttnArgs& a, const Scope& s, 
 // lines where the queries lie in one block of the part.  (8 x 17 rows of 32 heads: 8.2
 // us, 10.4 with a row's places and heads by neighbouring threads, 64 bytes together.
 // Six parts' loads in flight: with 3 or 12 the same, or up to 2 us more.)
-template <int DT, int D>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
+// Many parts (few rows over a long prefix) are shared out over kGroups times as many
+// threads, whose sums meet in LDS.
+template <int DT, int D, int kGroups>
+__global__ __launch_bounds__(kJoinThreads* kGroups) void join_kernel(AttnArgs a) {
     constexpr int kBatch = 6;
-    const int per_kv = a.heads / a.cache.kv_heads;
-    const int d = int(blockIdx.x % (D / 32)) * 32 + int(threadIdx.x / 32) * 4;
+    __shared__ float other[kGroups > 1 ? kGroups - 1 : 1][6][kGroups > 1 ? kJoinThreads : 1];
+    const int per_kv = a.heads / a.cache.kv_heads, group = int(threadIdx.x / kJoinThreads), t = int(threadIdx.x % kJoinThreads);
+    const int d = int(blockIdx.x % (D / 32)) * 32 + t / 32 * 4;
     const int kv = int(blockIdx.x / (D / 32) % unsigned(a.cache.kv_heads));
-    const int64_t query = int64_t(blockIdx.x / (D / 32) / unsigned(a.cache.kv_heads)) * 32 + threadIdx.x % 32;
+    const int64_t query = int64_t(blockIdx.x / (D / 32) / unsigned(a.cache.kv_heads)) * 32 + t % 32;
     const int row = int(query / per_kv), g = int(query % per_kv), head = kv * per_kv + g;
     RowInfo r = a.info[min(row, a.lanes.rows - 1)];   // (requested beside the number of rows)
     asm volatile("" ::: "memory");
-    if (row >= a.lanes.rows || row >= a.lanes.row_offsets[a.lanes.lanes]) return;
+    const bool live = row < a.lanes.rows && row < a.lanes.row_offsets[a.lanes.lanes];
+    if (kGroups == 1 && !live) return;
     // (a row that no lane holds, of offsets that do not begin at 0 or fall, has whatever lay there)
     r.own_parts = min(r.own_parts, a.plan.own.splits);
     r.group_parts = min(r.group_parts, r.group < 0 ? 0 : a.plan.prefix.splits);
@@ -724,7 +729,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
         r.lost = 1;
     float top = -kInfF, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
-    if (!r.lost) {
+    if (live && !r.lost) {
         // the group's parts, then the lane's own, kBatch parts' loads in flight
         int64_t first[2], step[2];
         int m[2];
@@ -736,8 +741,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
             step[k] = part_block(a, !k, 1, which, kv) + m[k] / 32 - first[k];
         }
         const int place = (d / 8 * 2 + (d / 4 & 1)) * 32;   // of a block, in float4
-        const int parts = r.group_parts + r.own_parts;
-        for (int i0 = 0; i0 < parts; i0 += kBatch) {
+        const int all = r.group_parts + r.own_parts, each = (all + kGroups - 1) / kGroups;
+        const int parts = min(all, (group + 1) * each);
+        for (int i0 = group * each; i0 < parts; i0 += kBatch) {
             float2 ml[kBatch];
             float4 v[kBatch];
 #pragma unroll
@@ -770,6 +776,26 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
     } else {
         sum = __builtin_nanf("");
     }
+    if constexpr (kGroups > 1) {
+        if (group > 0) {
+            const float left[6] = {top, sum, o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int k = 0; k < 6; ++k) other[group - 1][k][t] = left[k];
+        }
+        __syncthreads();
+        if (group > 0 || !live) return;
+#pragma unroll
+        for (int k = 0; k < kGroups - 1; ++k) {
+            const float ot = other[k][0][t], os = other[k][1][t];
+            if (ot == -kInfF && os == 0.0f) continue;   // its parts saw nothing
+            const float next = fmaxf(top, ot);
+            const float x = rescale(top, next, a.scale2), y = rescale(ot, next, a.scale2);
+            top = next;
+            sum = sum * x + os * y;
+            o.x = o.x * x + other[k][2][t] * y; o.y = o.y * x + other[k][3][t] * y;
+            o.z = o.z * x + other[k][4][t] * y; o.w = o.w * x + other[k][5][t] * y;
+        }
+    }
     const bool empty = sum == 0.0f;
     const float inv = empty ? 0.0f : 1.0f / sum;
     uint16_t* const out = static_cast<uint16_t*>(a.out) + int64_t(row) * a.out_row + int64_t(head) * a.out_head + d;
@@ -801,17 +827,25 @@ AttnPlan attention_plan(int heads, int kv_heads, int head_dim, int lanes, int gr
     // is left, in parts of at most 704 keys that fill the gaps.  64 x 1 rows over 32,768 shared
     // and 2,048 own keys, 8 kv heads: 144 us so, 155 with own parts of 2,112 keys, 172 with
     // two prefix parts a CU; the prefix alone 99 us with two parts a CU.
-    const int64_t slots = int64_t(device_cus()) * (head_dim == 256 ? 1 : 2), least = 2 * tile;
+    const int64_t slots = int64_t(device_cus()) * (head_dim == 256 ? 1 : 2);
     const int64_t own_work = own_items * max_own, prefix_work = prefix_items * max_prefix;
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    // Few items over many keys: a part costs the join about two fifths of what a tile costs
+    // the part, so both together are least near sqrt(tiles / 2.5) tiles a part (two at least).
+    // 12 x 1 rows of 4 heads of 128 places over 21,312 shared keys: 27 us so, 33 with two tiles a
+    // part, 30 with four; 1 row of 16 heads of 256 over 10,608: 37, 47 and 46.
+    auto most_parts = [&](int64_t keys) {
+        const int64_t tiles = up(keys, tile);
+        return up(tiles, std::max<int64_t>(2, std::llround(std::sqrt(double(tiles) / 2.5))));
+    };
     int64_t prefix_splits = 0;
     if (groups) {
         const int64_t share = own_work * 8 < prefix_work ? slots : std::max<int64_t>(slots / 2, 1);
-        prefix_splits = std::clamp<int64_t>(std::min(share / prefix_items, up(max_prefix, least)), 1, 128);
+        prefix_splits = std::clamp<int64_t>(std::min(share / prefix_items, most_parts(max_prefix)), 1, 128);
     }
     const int64_t rest = std::max<int64_t>(slots - prefix_items * prefix_splits, 1);
     const int64_t own_splits =
-        std::clamp<int64_t>(std::min(std::max(rest / own_items, up(max_own, 704)), up(max_own, least)), 1, 128);
+        std::clamp<int64_t>(std::min(std::max(rest / own_items, up(max_own, 704)), most_parts(max_own)), 1, 128);
     auto cut = [&](ScopePlan& scope, int64_t keys, int64_t n) {   // into chunks alike
         scope.splits = int(n);
         const int64_t each = (std::max<int64_t>(keys, 1) + scope.splits - 1) / scope.splits;
@@ -827,6 +861,10 @@ size_t attention_blocks(const AttnPlan& p, int kv_heads, int lanes, int groups) 
                                size_t(p.prefix.splits) * groups * p.prefix.tiles * p.prefix.waves);
 }
 
+// Parts of a row that one thread a place joins; the join of more takes four (the same two
+// cases: 33 us and 47, with one thread 42 and 61; the twelve parts and fewer of larger
+// batches take as long either way).
+constexpr int kFewParts = 12;
 int64_t join_blocks(const AttnArgs& a) {
     const int64_t queries = int64_t(a.lanes.rows) * (a.heads / a.cache.kv_heads);
     return (queries + 31) / 32 * a.cache.kv_heads * (a.cache.head_dim / 32);
@@ -834,7 +872,11 @@ int64_t join_blocks(const AttnArgs& a) {
 
 template <int DT, int D> void launch_dim(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     hipLaunchKernelGGL((attend_kernel<DT, D>), dim3(blocks), dim3(Tile<D>::kWaves * kWave), 0, stream, a);
-    hipLaunchKernelGGL((join_kernel<DT, D>), dim3(unsigned(join_blocks(a))), dim3(kJoinThreads), 0, stream, a);
+    const dim3 joins{unsigned(join_blocks(a))};
+    if (a.plan.prefix.splits + a.plan.own.splits > kFewParts)
+        hipLaunchKernelGGL((join_kernel<DT, D, 4>), joins, dim3(4 * kJoinThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((join_kernel<DT, D, 1>), joins, dim3(kJoinThreads), 0, stream, a);
 }
 template <int DT> void launch_type(const AttnArgs& a, unsigned blocks, hipStream_t stream) {
     switch (a.cache.head_dim) {
