@@ -316,3 +316,41 @@ def test_refusals(dev):
     with pytest.raises(vi.VIError):      # a head size that has no kernel
         vi.prefix_attention(torch.zeros(2, 4, 96, dtype=torch.float16, device=dev), *(torch.zeros(
             3, 2, 16, 96, dtype=torch.float16, device=dev) for _ in range(2)), *base[3:], **ok)
+
+
+@BOTH
+@pytest.mark.parametrize("counts,contexts,heads,kv,dim,page,groups", [
+    ([1], [9000], 4, 1, 128, 16, ()),
+    ([1, 3], [7001, 6500], 6, 2, 64, 32, [(2, 6400)]),
+    ([2, 1], [5003, 4100], 7, 1, 256, 64, [(1, 5000), (1, 0)]),
+])
+def test_many_parts(dev, rng, dtype, counts, contexts, heads, kv, dim, page, groups):
+    """Few rows over many keys: more parts than one thread joins.  A first and a last part that hold what no
+    number is, a part without a page, rows past the last lane and rows past the bounds."""
+    c = Case(rng, dev, dtype, counts, contexts, heads, kv, dim, page, groups)
+    good = c.run().clone()
+    c.check(good)
+    # padding rows stay as they are
+    q, out = c.q, torch.full((q_rows := c.q.shape[0] + 3, heads, dim), 5.0, dtype=dtype, device=dev)
+    c.q = torch.cat([q, q[:1].expand(3, -1, -1)])
+    c.run(out=out)
+    assert torch.equal(out[:q_rows - 3], good) and bool((out[q_rows - 3:] == 5).all()) and bool((c.lse[q_rows - 3:] == 7).all())
+    c.q = q
+    # an infinite value of the last lane's last row: seen by that row alone, in one place
+    l = len(counts) - 1
+    at = contexts[l] + counts[l] - 1
+    page_of, place = c.tables[l, at // page], at % page
+    keep = c.pool[1, page_of, 0, place, 3].clone()
+    c.pool[1, page_of, 0, place, 3] = float("inf")
+    out = c.run()
+    c.pool[1, page_of, 0, place, 3] = keep
+    per = heads // kv
+    assert bool((out[-1, :per, 3] == float("inf")).all())
+    out[-1, :per, 3] = good[-1, :per, 3]
+    assert torch.equal(out, good)
+    # a token in the middle without a page
+    e = (contexts[l] // 2 // page) if not groups or groups[-1][1] == 0 else (contexts[l] - 5) // page
+    c.tables[l, e] = -1
+    out = c.run()
+    n = counts[l]
+    assert bool(torch.isnan(out[-n:]).all()) and torch.equal(out[:-n], good[:-n])
